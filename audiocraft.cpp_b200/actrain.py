@@ -19,7 +19,8 @@ LIB_PATH = os.path.join(HERE, "libactrain.so")
 ACT_OK, ACT_ERR_INVALID, ACT_ERR_CUDA, ACT_ERR_NCCL, ACT_ERR_STATE, ACT_ERR_NONFINITE = range(6)
 FAMILY_MELODYFLOW, FAMILY_MUSICGEN = 0, 1
 ADAPTER_LORA, ADAPTER_DORA_ROWS = 0, 1
-TYPE_F32, TYPE_F16, TYPE_Q8_0 = 0, 1, 8
+TYPE_F32, TYPE_F16, TYPE_Q8_0, TYPE_BF16 = 0, 1, 8, 30
+CKPT_I8, CKPT_E4M3 = 1, 2
 TARGETS = ("self.qkv", "self.out", "cross.q", "cross.kv", "cross.out", "ff.0", "ff.2")
 # kernel families counted by act_path_counts (ACT_PATH_*)
 PATHS = ("attn_fwd_tc", "attn_fwd_mma", "attn_bwd_tc", "attn_bwd_mma", "gemm_tc", "gemm_mma", "rank_tc",
@@ -56,6 +57,11 @@ class Opt(C.Structure):
     _fields_ = [("lr", C.c_float), ("beta1", C.c_float), ("beta2", C.c_float), ("eps", C.c_float),
                 ("weight_decay", C.c_float), ("clip", C.c_float), ("step", C.c_int),
                 ("count", C.c_int)]
+
+
+class Ckpt8(C.Structure):
+    _fields_ = [("type", C.c_int), ("q", C.c_void_p), ("ldq", C.c_int64), ("scale", C.c_void_p),
+                ("lds", C.c_int64)]
 
 
 class ActError(RuntimeError):
@@ -117,6 +123,24 @@ SIGNATURES = {
     "act_mf_staged": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t]),
     "act_lora_linear": (C.c_int, [C.c_int, C.c_void_p, C.c_int64, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_size_t,
                                   C.c_void_p, C.c_void_p, C.c_int, C.c_float, C.c_void_p, C.c_float, C.c_void_p]),
+    "act_ckpt8_store": (C.c_int, [C.c_void_p, C.c_int] + [C.c_int64] * 3 + [C.c_int, C.POINTER(Ckpt8), C.c_void_p]),
+    "act_ckpt8_load": (C.c_int, [C.POINTER(Ckpt8), C.c_int64, C.c_int64, C.c_int, C.c_void_p, C.c_int, C.c_int64,
+                                 C.c_void_p]),
+    "act_layernorm_fwd": (C.c_int, [C.c_void_p, C.c_int] + [C.c_int64] * 3 + [C.c_void_p, C.c_void_p, C.c_float,
+                                    C.c_void_p, C.c_int, C.c_int64, C.POINTER(Ckpt8), C.c_void_p, C.c_void_p,
+                                    C.POINTER(Ckpt8), C.c_void_p]),
+    "act_layernorm_bwd": (C.c_int, [C.c_void_p, C.c_int, C.c_int64] * 2 + [C.POINTER(Ckpt8)] + [C.c_void_p] * 3 +
+                          [C.c_int64, C.c_int64, C.c_void_p, C.c_void_p, C.c_int, C.c_int64, C.c_void_p, C.c_void_p,
+                           C.c_int, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "act_layernorm_bwd_workspace": (C.c_int64, [C.c_int64, C.c_int64]),
+    "act_gelu_ckpt8_fwd": (C.c_int, [C.c_void_p, C.c_int] + [C.c_int64] * 3 + [C.c_void_p, C.c_int64,
+                                     C.POINTER(Ckpt8), C.POINTER(Ckpt8), C.c_void_p]),
+    "act_gelu_ckpt8_bwd": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.POINTER(Ckpt8), C.c_int64, C.c_int64,
+                                     C.c_void_p, C.c_int64, C.POINTER(Ckpt8), C.c_void_p]),
+    "act_rank_gemm_ckpt8": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_int, C.POINTER(Ckpt8), C.c_int64, C.c_int64,
+                                      C.c_float, C.c_void_p, C.c_int64, C.c_int, C.c_void_p, C.c_void_p]),
+    "act_gemm_f8": (C.c_int, [C.POINTER(Ckpt8), C.POINTER(Ckpt8)] + [C.c_int64] * 3 + [C.c_int, C.c_void_p, C.c_void_p,
+                              C.c_int, C.c_int64, C.c_int, C.c_void_p, C.c_void_p]),
     "act_rank_gemm_f16": (C.c_int, [C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int,
                                      C.c_int, C.c_int, C.c_float, C.c_int, C.c_int, C.POINTER(C.c_float)]),
     "act_rank_gemm_q8_0": (C.c_int, [C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int,
@@ -487,6 +511,84 @@ def attention_bwd_noalloc(q, k, v, o, lse, dout, dq, dk, dv, clips, T, Tk, H, nv
                                          int(causal), int(zero_key), rope or None, stream or None)
     if rc != ACT_OK:
         raise ActError(rc, lib().act_last_error(None).decode())
+
+
+# ----------------------------------------------------------------- 8-bit checkpoints, layer norm, 8-bit GEMM
+# Every tensor argument below is a device address (int, 0 for NULL); ld = 0 means dense rows; a
+# Ckpt8 is passed as such or as None.  Work is queued on `stream` (0: the legacy default stream).
+def ckpt8(type: int, q: int, ldq: int, scale: int, lds: int) -> Ckpt8:
+    """An 8-bit tensor by device addresses: codes (row stride ldq bytes) and block-major scales
+    [ceil(cols / 128)][lds]."""
+    return Ckpt8(type, q, ldq, scale, lds)
+
+
+def _call(rc):
+    if rc != ACT_OK:
+        raise ActError(rc, lib().act_last_error(None).decode())
+
+
+def _ref(view):
+    return None if view is None else C.byref(view)
+
+
+def ckpt8_store(x, x_type, rows, cols, out, block_rows=1, ldx=0, stream=0):
+    """act_ckpt8_store: x [rows][cols] in 8 bits, blocks of 128 columns x block_rows (1 or 128) rows."""
+    _call(lib().act_ckpt8_store(x, x_type, ldx or cols, rows, cols, block_rows, _ref(out), stream))
+
+
+def ckpt8_load(src, rows, cols, y, y_type, block_rows=1, ldy=0, stream=0):
+    """act_ckpt8_load: the values an 8-bit tensor stands for, rounded to y_type."""
+    _call(lib().act_ckpt8_load(_ref(src), rows, cols, block_rows, y, y_type, ldy or cols, stream))
+
+
+def layernorm_fwd(x, x_type, rows, dim, w, b, y, y_type, mean, rstd, eps=1e-5, ldx=0, ldy=0, y8=None, x8=None,
+                  stream=0):
+    """act_layernorm_fwd: y (and y8, its 8-bit form), row statistics, and x8, the 8-bit checkpoint of x."""
+    _call(lib().act_layernorm_fwd(x, x_type, ldx or dim, rows, dim, w, b, eps, y, y_type, ldy or dim, _ref(y8), mean,
+                                  rstd, _ref(x8), stream))
+
+
+def layernorm_bwd_workspace(rows, dim) -> int:
+    """Bytes of workspace act_layernorm_bwd needs for this shape on the current device."""
+    n = int(lib().act_layernorm_bwd_workspace(rows, dim))
+    if n < 0:
+        _call(ACT_ERR_INVALID)
+    return n
+
+
+def layernorm_bwd(dy, dy_type, x, x_type, w, mean, rstd, rows, dim, dx, dx_type, dw, db, workspace, workspace_bytes,
+                  accumulate=False, add=0, x8=None, lddy=0, ldx=0, lddx=0, stream=0):
+    """act_layernorm_bwd: dx, and the sums over the rows dw and db; x = 0 reads the checkpoint x8 instead."""
+    _call(lib().act_layernorm_bwd(dy, dy_type, lddy or dim, x, x_type, ldx or dim, _ref(x8), w, mean, rstd, rows, dim,
+                                  add, dx, dx_type, lddx or dim, dw, db, int(accumulate), workspace, workspace_bytes,
+                                  stream))
+
+
+def gelu_ckpt8_fwd(z, z_type, rows, cols, g, g_type, z8, g8=None, ldz=0, ldg=0, stream=0):
+    """act_gelu_ckpt8_fwd: g (and g8) = GELU(z), z8 = the 8-bit checkpoint of z; g_type is z_type."""
+    if g_type != z_type:
+        raise ActError(ACT_ERR_INVALID, "gelu_ckpt8_fwd: g has z's type")
+    _call(lib().act_gelu_ckpt8_fwd(z, z_type, ldz or cols, rows, cols, g, ldg or cols, _ref(g8), _ref(z8), stream))
+
+
+def gelu_ckpt8_bwd(dg, dg_type, z8, rows, cols, dz, dz_type, dz8=None, lddg=0, lddz=0, stream=0):
+    """act_gelu_ckpt8_bwd: dz (and dz8) = dg * GELU'(kept z); dz_type is dg_type."""
+    if dz_type != dg_type:
+        raise ActError(ACT_ERR_INVALID, "gelu_ckpt8_bwd: dz has dg's type")
+    _call(lib().act_gelu_ckpt8_bwd(dg, dg_type, lddg or cols, _ref(z8), rows, cols, dz, lddz or cols, _ref(dz8),
+                                   stream))
+
+
+def rank_gemm_ckpt8(u, u_type, nb, x8, rows, cols, c, status, alpha=1.0, accumulate=False, ldu=0, ldc=0, stream=0):
+    """act_rank_gemm_ckpt8: C [nb][cols] (+)= alpha * U^T X with X an 8-bit tensor [rows][cols]."""
+    _call(lib().act_rank_gemm_ckpt8(u, u_type, ldu or nb, nb, _ref(x8), rows, cols, alpha, c, ldc or cols,
+                                    int(accumulate), status, stream))
+
+
+def gemm_f8(x8, w8, M, N, K, y, y_type, status, w_mn_major=False, bias=0, accumulate=False, ldy=0, stream=0):
+    """act_gemm_f8: Y [M][N] (+)= X8 W8^T (+ bias), W8 [N][K] or, with w_mn_major, [K][N]."""
+    _call(lib().act_gemm_f8(_ref(x8), _ref(w8), M, N, K, int(w_mn_major), bias, y, y_type, ldy or N, int(accumulate),
+                            status, stream))
 
 
 def mf_model(dim, layers, heads, ff_dim, latent_dim=128, cond_dim=768, time_dim=256, norm_eps=1e-5):

@@ -1,0 +1,266 @@
+// ckpt8.cu -- activations put away in 8 bits and read back, alone and inside the GELU's forward
+// and backward passes.
+//
+// Every kernel here is one pass over its tensors and bound by HBM: store reads 4 or 2 bytes an
+// element and writes 1 (+ 4 bytes a block), load the reverse; the GELU's forward reads 2 and
+// writes 2 + 1, its backward reads 2 + 1 and writes 2 (16-bit types).  A warp takes one block of
+// 128 columns and RPW neighbouring rows of it at a time: the block's maximum is one warp
+// reduction, the loads of all rows are in flight together, and the rows' scales, which lie next
+// to each other (block-major), leave as one store.
+#include "ckpt8.cuh"
+
+namespace act {
+
+namespace {
+
+using namespace c8;
+
+constexpr int RPW = 4;        // rows of a block column a warp holds at a time
+constexpr int THREADS = 256;
+
+// A warp's block column and its first row group; warps beyond the last whole set of block
+// columns have none
+struct Place {
+    int chunk, n;    // block column, columns of the row from its first one
+    long row, step;  // first row, rows between two groups of this warp
+    bool any;
+};
+__device__ __forceinline__ Place place(long rows, long cols) {
+    const unsigned warp = blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5), nwarps = gridDim.x * (THREADS / 32);
+    const unsigned chunks = (unsigned)((cols + BLOCK - 1) / BLOCK), lanes = nwarps / chunks;
+    Place p;
+    p.chunk = (int)(warp % chunks);
+    p.row = (long)(warp / chunks) * RPW;
+    p.step = (long)lanes * RPW;
+    p.any = warp / chunks < lanes;
+    const long left = cols - (long)p.chunk * BLOCK;
+    p.n = left < BLOCK ? (int)left : BLOCK;
+    return p;
+}
+
+// the scales of up to RPW rows: lane r holds row r's
+__device__ __forceinline__ void store_scales(const Q8& t, int chunk, long row, int nr, int lane, const uint32_t* s) {
+    uint32_t mine = s[0];
+#pragma unroll
+    for (int r = 1; r < RPW; ++r) mine = lane == r ? s[r] : mine;
+    if (lane < nr) t.scale[(long)chunk * t.lds + row + lane] = __uint_as_float(mine);
+}
+
+template <typename T, bool VEC, bool E4M3>
+__global__ void __launch_bounds__(THREADS) store_kernel(const T* x, long ldx, long rows, long cols, Q8 out) {
+    const int lane = threadIdx.x & 31;
+    const Place p = place(rows, cols);
+    if (!p.any) return;
+    const long c0 = (long)p.chunk * BLOCK;
+    for (long row = p.row; row < rows; row += p.step) {
+        const int nr = rows - row < RPW ? (int)(rows - row) : RPW;
+        float v[RPW][4];
+        uint32_t s[RPW];
+#pragma unroll
+        for (int r = 0; r < RPW; ++r) load4<T, VEC>(x + (row + r) * ldx + c0, r < nr ? p.n : 0, lane, v[r]);
+#pragma unroll
+        for (int r = 0; r < RPW; ++r)
+            s[r] = store_block<VEC>(out.q + (row + r) * out.ldq + c0, r < nr ? p.n : 0, lane, v[r], E4M3);
+        store_scales(out, p.chunk, row, nr, lane, s);
+    }
+}
+
+// one CTA per 128 x 128 block: a first pass for the maximum, a second that finds the block in L1
+template <typename T, bool VEC, bool E4M3>
+__global__ void __launch_bounds__(THREADS) store_square_kernel(const T* x, long ldx, long rows, long cols, Q8 out) {
+    __shared__ uint32_t top[THREADS / 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const long c0 = (long)blockIdx.x * BLOCK;
+    const int n = cols - c0 < BLOCK ? (int)(cols - c0) : BLOCK;
+    for (long rb = blockIdx.y; rb * BLOCK < rows; rb += gridDim.y) {
+        const long r0 = rb * BLOCK, r1 = r0 + BLOCK < rows ? r0 + BLOCK : rows;
+        uint32_t m = 0, any = 0;
+        for (long r = r0 + warp; r < r1; r += THREADS / 32) {
+            float v[4];
+            load4<T, VEC>(x + r * ldx + c0, n, lane, v);
+            m = max(m, largest_finite(v));
+            any = max(any, largest(v));
+        }
+        const bool bad = __syncthreads_or(any >= 0x7f800000u);
+        m = __reduce_max_sync(FULL, m);
+        if (lane == 0) top[warp] = m;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < THREADS / 32; ++w) m = max(m, top[w]);
+        const uint32_t s = scale_bits(m, E4M3);
+        for (long r = r0 + warp; r < r1; r += THREADS / 32) {
+            float v[4];
+            load4<T, VEC>(x + r * ldx + c0, n, lane, v);
+            store_codes<VEC>(out.q + r * out.ldq + c0, n, lane, encode4(v, inverse_pow2(s), E4M3, bad));
+        }
+        if (threadIdx.x == 0) out.scale[(long)blockIdx.x * out.lds + rb] = __uint_as_float(s);
+    }
+}
+
+// shift: log2 of the block's rows
+template <typename T, bool VEC, bool E4M3>
+__global__ void __launch_bounds__(THREADS) load_kernel(Q8 in, long rows, long cols, int shift, T* y, long ldy) {
+    const int lane = threadIdx.x & 31;
+    const Place p = place(rows, cols);
+    if (!p.any) return;
+    const long c0 = (long)p.chunk * BLOCK;
+    for (long row = p.row; row < rows; row += p.step) {
+        const int nr = rows - row < RPW ? (int)(rows - row) : RPW;
+        float v[RPW][4], s[RPW];
+        uint32_t w[RPW];
+#pragma unroll
+        for (int r = 0; r < RPW; ++r) {
+            w[r] = load_codes<VEC>(in.q + (row + r) * in.ldq + c0, r < nr ? p.n : 0, lane);
+            s[r] = r < nr ? in.scale[(long)p.chunk * in.lds + ((row + r) >> shift)] : 0.f;
+        }
+#pragma unroll
+        for (int r = 0; r < RPW; ++r) {
+            decode4(w[r], E4M3, v[r]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[r][i] *= s[r];
+            store4<T, VEC>(y + (row + r) * ldy + c0, r < nr ? p.n : 0, lane, v[r]);
+        }
+    }
+}
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(THREADS)
+    gelu_fwd_kernel(const T* z, long ldz, long rows, long cols, T* g, long ldg, Q8 g8, Q8 z8) {
+    const int lane = threadIdx.x & 31;
+    const Place p = place(rows, cols);
+    if (!p.any) return;
+    const long c0 = (long)p.chunk * BLOCK;
+    for (long row = p.row; row < rows; row += p.step) {
+        const int nr = rows - row < RPW ? (int)(rows - row) : RPW;
+        float v[RPW][4];
+        uint32_t s[RPW];
+#pragma unroll
+        for (int r = 0; r < RPW; ++r) load4<T, VEC>(z + (row + r) * ldz + c0, r < nr ? p.n : 0, lane, v[r]);
+#pragma unroll
+        for (int r = 0; r < RPW; ++r)
+            s[r] = store_block<VEC>(z8.q + (row + r) * z8.ldq + c0, r < nr ? p.n : 0, lane, v[r], z8.e4m3);
+        store_scales(z8, p.chunk, row, nr, lane, s);
+#pragma unroll
+        for (int r = 0; r < RPW; ++r) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[r][i] = gelu(v[r][i]);
+            if (g) store4<T, VEC>(g + (row + r) * ldg + c0, r < nr ? p.n : 0, lane, v[r]);
+        }
+        if (g8.q) {
+#pragma unroll
+            for (int r = 0; r < RPW; ++r)
+                s[r] = store_block<VEC>(g8.q + (row + r) * g8.ldq + c0, r < nr ? p.n : 0, lane, v[r], g8.e4m3);
+            store_scales(g8, p.chunk, row, nr, lane, s);
+        }
+    }
+}
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(THREADS)
+    gelu_bwd_kernel(const T* dg, long lddg, Q8 z8, long rows, long cols, T* dz, long lddz, Q8 dz8) {
+    const int lane = threadIdx.x & 31;
+    const Place p = place(rows, cols);
+    if (!p.any) return;
+    const long c0 = (long)p.chunk * BLOCK;
+    for (long row = p.row; row < rows; row += p.step) {
+        const int nr = rows - row < RPW ? (int)(rows - row) : RPW;
+        float v[RPW][4], s[RPW];
+        uint32_t w[RPW];
+#pragma unroll
+        for (int r = 0; r < RPW; ++r) {
+            load4<T, VEC>(dg + (row + r) * lddg + c0, r < nr ? p.n : 0, lane, v[r]);
+            w[r] = load_codes<VEC>(z8.q + (row + r) * z8.ldq + c0, r < nr ? p.n : 0, lane);
+            s[r] = r < nr ? z8.scale[(long)p.chunk * z8.lds + row + r] : 0.f;
+        }
+#pragma unroll
+        for (int r = 0; r < RPW; ++r) {
+            float z[4];
+            decode4(w[r], z8.e4m3, z);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[r][i] *= gelu_grad(z[i] * s[r]);
+            if (dz) store4<T, VEC>(dz + (row + r) * lddz + c0, r < nr ? p.n : 0, lane, v[r]);
+        }
+        if (dz8.q) {
+            uint32_t sb[RPW];
+#pragma unroll
+            for (int r = 0; r < RPW; ++r)
+                sb[r] = store_block<VEC>(dz8.q + (row + r) * dz8.ldq + c0, r < nr ? p.n : 0, lane, v[r], dz8.e4m3);
+            store_scales(dz8, p.chunk, row, nr, lane, sb);
+        }
+    }
+}
+
+// enough warps to fill the GPU (eight CTAs of 256 an SM) or, if there is less, one row group each;
+// at least one warp per block column
+int grid_for(long rows, long cols) {
+    const long chunks = (cols + BLOCK - 1) / BLOCK, groups = (rows + RPW - 1) / RPW;
+    const long per = THREADS / 32, full = (long)current_sm_count() * 8 * per;
+    long warps = chunks * groups;
+    if (warps > full) warps = full > chunks ? full : chunks;
+    return (int)((warps + per - 1) / per);
+}
+
+template <typename T>
+T* as(const OpTensor& t) {
+    return static_cast<T*>(const_cast<void*>(t.p));
+}
+
+// f(T{}) with T the element type
+template <typename Fn>
+void by_type(int type, Fn&& f) {
+    if (type == OP_F16) f(f16{});
+    else if (type == OP_BF16) f(__nv_bfloat16{});
+    else f(float{});
+}
+
+}  // namespace
+
+void ckpt8_store(const OpTensor& x, long rows, long cols, int block_rows, const Q8& out, cudaStream_t s) {
+    const bool v = vec4(x) && vec4(out);
+    by_type(x.type, [&](auto t) {
+        typedef decltype(t) T;
+        if (block_rows == 1) {
+            auto* k = v ? (out.e4m3 ? store_kernel<T, true, true> : store_kernel<T, true, false>)
+                        : (out.e4m3 ? store_kernel<T, false, true> : store_kernel<T, false, false>);
+            k<<<grid_for(rows, cols), THREADS, 0, s>>>(as<const T>(x), x.ld, rows, cols, out);
+        } else {
+            auto* k = v ? (out.e4m3 ? store_square_kernel<T, true, true> : store_square_kernel<T, true, false>)
+                        : (out.e4m3 ? store_square_kernel<T, false, true> : store_square_kernel<T, false, false>);
+            const long rb = (rows + BLOCK - 1) / BLOCK;
+            k<<<dim3((unsigned)((cols + BLOCK - 1) / BLOCK), (unsigned)(rb < 65535 ? rb : 65535)), THREADS, 0, s>>>(
+                as<const T>(x), x.ld, rows, cols, out);
+        }
+    });
+}
+
+void ckpt8_load(const Q8& in, long rows, long cols, int block_rows, const OpTensor& y, cudaStream_t s) {
+    const bool v = vec4(y) && vec4(in);
+    by_type(y.type, [&](auto t) {
+        typedef decltype(t) T;
+        auto* k = v ? (in.e4m3 ? load_kernel<T, true, true> : load_kernel<T, true, false>)
+                    : (in.e4m3 ? load_kernel<T, false, true> : load_kernel<T, false, false>);
+        k<<<grid_for(rows, cols), THREADS, 0, s>>>(in, rows, cols, block_rows == 1 ? 0 : 7, as<T>(y), y.ld);
+    });
+}
+
+void gelu_ckpt8_fwd(const OpTensor& z, long rows, long cols, const OpTensor& g, const Q8& g8, const Q8& z8,
+                    cudaStream_t s) {
+    const bool v = vec4(z) && vec4(g) && vec4(g8) && vec4(z8);
+    by_type(z.type, [&](auto t) {
+        typedef decltype(t) T;
+        auto* k = v ? gelu_fwd_kernel<T, true> : gelu_fwd_kernel<T, false>;
+        k<<<grid_for(rows, cols), THREADS, 0, s>>>(as<const T>(z), z.ld, rows, cols, as<T>(g), g.ld, g8, z8);
+    });
+}
+
+void gelu_ckpt8_bwd(const OpTensor& dg, const Q8& z8, long rows, long cols, const OpTensor& dz, const Q8& dz8,
+                    cudaStream_t s) {
+    const bool v = vec4(dg) && vec4(dz) && vec4(z8) && vec4(dz8);
+    by_type(dg.type, [&](auto t) {
+        typedef decltype(t) T;
+        auto* k = v ? gelu_bwd_kernel<T, true> : gelu_bwd_kernel<T, false>;
+        k<<<grid_for(rows, cols), THREADS, 0, s>>>(as<const T>(dg), dg.ld, z8, rows, cols, as<T>(dz), dz.ld, dz8);
+    });
+}
+
+}  // namespace act

@@ -44,6 +44,7 @@ extern "C" {
 #define ACT_TYPE_F32 0
 #define ACT_TYPE_F16 1
 #define ACT_TYPE_Q8_0 8
+#define ACT_TYPE_BF16 30 /* the 8-bit checkpoint, layer norm and 8-bit GEMM entry points below only */
 
 /* adapter target bits, in the reference's order (src/mf/train.h:69, src/mg/train.h:90) */
 #define ACT_TARGET_SELF_QKV (1u << 0)
@@ -319,6 +320,97 @@ int64_t act_graph_kernel_nodes(act_ctx* ctx, int n);
 int act_lora_linear(int device, const float* x, int64_t rows, int in, int out, int w_type, const void* w,
                     size_t w_bytes, const float* A, const float* B, int rank, float alpha, const float* magnitude,
                     float strength, float* y);
+
+/* ---- layer norm with weight gradients, 8-bit activation checkpoints, 8-bit GEMM ----
+ * Operators for training more than the adapters keep today: norms whose weight and bias learn,
+ * activations kept in 8 bits between forward and backward, and projections whose two operands
+ * are 8-bit floating point.  No counterpart in the reference (its norms are frozen, its
+ * activations fp32, src/mf/dit.h and src/ac/lora.h).
+ *
+ * Every pointer is a DEVICE pointer of the calling thread's current device (checked: a host
+ * pointer or another device's is rejected), work is queued asynchronously on `stream` (NULL =
+ * the legacy default stream), nothing is allocated, and every call may be captured into a CUDA
+ * graph.  Tensors are row-major with a row stride in elements (ld >= columns); element types are
+ * ACT_TYPE_F32, ACT_TYPE_F16 and ACT_TYPE_BF16, and base pointers are aligned to the element.
+ * Any stride and alignment is taken; vectors move when bases and strides are multiples of four
+ * elements.  Outputs must not overlap inputs unless said otherwise.  rows = 0 does nothing (and
+ * zeroes sums over the rows that are not accumulated).  The same call gives the same bits every
+ * time on the same GPU model: no reduction depends on the order in which blocks finish.
+ *
+ * An 8-bit tensor is codes and scales.  A block is 128 neighbouring columns (the last one of a
+ * row may be shorter) of one row, or of 128 rows for a weight, and has one fp32 scale: the
+ * smallest power of two s >= 2^-126 with |x| <= top * s for every finite x of the block (top 448
+ * for E4M3, 127 for I8; an all-zero block has 2^-126).  A code is x / s rounded to nearest even,
+ * which is exact arithmetic: codes and scales depend on x alone.  Relative to a free scale the
+ * power of two costs E4M3 nothing but subnormal range, and I8 at most one bit.  A value that is
+ * not finite is stored as NaN (E4M3 code 0x7f, I8 code -128) and leaves its block's scale alone.
+ * Scales lie block-major, scale[(column / 128) * lds + row] (row / 128 for blocks of 128 rows):
+ * the order in which both products read them. */
+#define ACT_CKPT_I8 1   /* whole numbers -127 .. 127: the smaller error, for checkpoints */
+#define ACT_CKPT_E4M3 2 /* 8-bit floating point: checkpoints, and operands of act_gemm_f8 */
+typedef struct {
+    int type;      /* ACT_CKPT_* */
+    void* q;       /* codes, one byte each, rows of ldq bytes */
+    int64_t ldq;
+    float* scale;  /* [ceil(columns / 128)][lds] */
+    int64_t lds;
+} act_ckpt8;
+
+/* x [rows][cols] -> codes and scales; block_rows 1 (activations) or 128 (weights) */
+int act_ckpt8_store(const void* x, int x_type, int64_t ldx, int64_t rows, int64_t cols, int block_rows,
+                    const act_ckpt8* out, void* stream);
+/* y [rows][cols] = the values codes and scales stand for, rounded to y_type */
+int act_ckpt8_load(const act_ckpt8* in, int64_t rows, int64_t cols, int block_rows, void* y, int y_type,
+                   int64_t ldy, void* stream);
+
+/* Layer norm of each row: mean, rstd = 1 / sqrt(variance + eps), y = (x - mean) * rstd * w + b in
+ * fp32, rounded once to y_type.  w and b are fp32 [dim], each may be NULL (1 and 0).  y may be
+ * NULL if y8 is given: y8 (E4M3 or I8, NULL to skip) receives the fp32 result in 8 bits, the
+ * operand of act_gemm_f8.  x8 (NULL to skip) receives x itself in 8 bits: the checkpoint
+ * act_layernorm_bwd reads in place of x.  mean and rstd are fp32 [rows].  dim <= 8192. */
+int act_layernorm_fwd(const void* x, int x_type, int64_t ldx, int64_t rows, int64_t dim, const float* w,
+                      const float* b, float eps, void* y, int y_type, int64_t ldy, const act_ckpt8* y8, float* mean,
+                      float* rstd, const act_ckpt8* x8, void* stream);
+/* Its backward pass, with h = (x - mean) * rstd and dh = dy * w:
+ *   dx = rstd * (dh - mean(dh) - h * mean(dh * h)) (+ add),   dw = sum over rows of dy * h,   db = sum of dy.
+ * x is given as it was (x_type, ldx) or, with x NULL, as the checkpoint x8.  add (NULL, or
+ * dx_type with row stride lddx; dx itself is allowed) is the gradient that reaches x past the
+ * norm.  dw and db are fp32 [dim], each may be NULL; accumulate 1 adds to what they hold.
+ * workspace: act_layernorm_bwd_workspace bytes, 16-byte aligned, free for reuse once the call's
+ * work is done: calls (and captured graphs) that overlap on the GPU need one each. */
+int act_layernorm_bwd(const void* dy, int dy_type, int64_t lddy, const void* x, int x_type, int64_t ldx,
+                      const act_ckpt8* x8, const float* w, const float* mean, const float* rstd, int64_t rows,
+                      int64_t dim, const void* add, void* dx, int dx_type, int64_t lddx, float* dw, float* db,
+                      int accumulate, void* workspace, size_t workspace_bytes, void* stream);
+/* bytes of workspace for that shape on the current device; -1 for a shape that is refused */
+int64_t act_layernorm_bwd_workspace(int64_t rows, int64_t dim);
+
+/* GELU with the checkpoint of its input: g = z * Phi(z) (Phi the normal distribution function),
+ * z8 receives z in 8 bits.  g may be NULL if g8 is given (fp32 result in 8 bits, as in
+ * act_layernorm_fwd).  g_type equals z_type. */
+int act_gelu_ckpt8_fwd(const void* z, int z_type, int64_t ldz, int64_t rows, int64_t cols, void* g, int64_t ldg,
+                       const act_ckpt8* g8, const act_ckpt8* z8, void* stream);
+/* dz = dg * (Phi(z) + z * phi(z)) at the kept z; dz of dg's type may be NULL if dz8 is given. dz may
+ * be dg itself. */
+int act_gelu_ckpt8_bwd(const void* dg, int dg_type, int64_t lddg, const act_ckpt8* z8, int64_t rows, int64_t cols,
+                       void* dz, int64_t lddz, const act_ckpt8* dz8, void* stream);
+
+/* Rank product with a checkpoint, the lora_A gradient (src/ac/lora.h:34-95) from a kept input:
+ *   C[j][c] (+)= alpha * sum over rows t of U[t][j] * X[t][c],   C fp32 [nb][cols], 1 <= nb <= 64.
+ * X in blocks of 1 row; its codes start on 16-byte boundaries (q and ldq multiples of 16).
+ * accumulate 0 overwrites C.  status: a device int that the caller zeroes once and may read at
+ * any time; nonzero means that a bounded wait inside the kernel ran out and C is not valid. */
+int act_rank_gemm_ckpt8(const void* u, int u_type, int64_t ldu, int nb, const act_ckpt8* x, int64_t rows,
+                        int64_t cols, float alpha, float* c, int64_t ldc, int accumulate, int32_t* status,
+                        void* stream);
+/* Product of two E4M3 tensors, X [M][K] in blocks of one row and W in blocks of 128 rows:
+ *   Y[m][n] = sum over k of X[m][k] * W[n][k] (+ bias[n]) (+ Y[m][n] with accumulate 1).
+ * W is stored [N][K] (w_mn_major 0: a projection) or [K][N] (1: the input gradient dY W of a
+ * weight [K = out][N = in], the same codes as the projection's).  Scales may be any fp32 values.
+ * Codes start on 16-byte boundaries (q and ldq multiples of 16).  bias fp32 [N] or NULL.  Sums are
+ * fp32.  status as in act_rank_gemm_ckpt8. */
+int act_gemm_f8(const act_ckpt8* x, const act_ckpt8* w, int64_t M, int64_t N, int64_t K, int w_mn_major,
+                const float* bias, void* y, int y_type, int64_t ldy, int accumulate, int32_t* status, void* stream);
 
 #if defined(__GNUC__)
 #pragma GCC visibility pop
