@@ -1,71 +1,412 @@
 // gemm_f8.cu -- product of two E4M3 tensors with a scale for each block of 128:
 //   Y[m][n] = sum over k-blocks b of sx[b][m] * sw[b][n / 128] * (sum over the block's k of X[m][k] W[n][k])
 //
-// A CTA owns 64 x 64 of Y; both operands are decoded on their way into shared memory, sums are
-// fp32 in registers.
+// The tensor cores take the codes as they are (tcgen05 kind::f8f6f4, fp32 accumulators in TMEM), one
+// k-block of 128 at a time; a block's scales are constant over it for each (row, 128 columns), so
+// its finished sum is multiplied by them once, in registers, on its way into the tile's sum.
+//
+// gemm_f8_kernel: one CTA per 128 x BN tile, persistent over tiles.  Warp 0 fills a ring of
+// k-blocks by TMA (128-byte swizzle; rows and columns past the tensor's end read as zero), one
+// thread of warp 1 issues four MMAs of 32 per k-block into one of two TMEM buffers, and eight
+// warps take turns with it: while the MMA of block i + 1 runs, they load block i from TMEM,
+// multiply-add it into 128 x BN fp32 sums held in registers (two columns per instruction) and
+// hand the buffer back.  A thread owns one row and half of the tile's columns.  The epilogue
+// turns the sums through shared memory, 32 columns at a time, so that global rows are written
+// in whole sectors; bias and the old value are added in fp32 before the one rounding.
+// Bound by the tensor cores for large M; the adding warps need about half of the MMA's time.
+//
+// gemm_f8_small_kernel: up to 16 rows (a few tokens).  Bound by reading W once: a CTA owns 16 rows
+// of W, its warps take every fourth k-block each, and the codes go straight from global memory
+// into mma.sync fragments: a lane loads 32 neighbouring codes of two rows of W and of its rows of
+// X, which is a fixed permutation of the block's k that both operands share.
+#include <cuda.h>
+
 #include "ckpt8.cuh"
+#include "tc_common.cuh"
 
 namespace act {
 
 namespace {
 
 using namespace c8;
+using namespace tc;
 
-__global__ void __launch_bounds__(256) gemm_f8_kernel(const GemmF8 p) {
-    __shared__ float xs[32][65], ws[32][65];
-    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    const long n0 = (long)blockIdx.x * 64;
-    for (long m0 = (long)blockIdx.y * 64; m0 < p.M; m0 += (long)gridDim.y * 64) {
-        float acc[4][4] = {};
-        for (long k0 = 0; k0 < p.K; k0 += 32) {
-            for (int i = threadIdx.x; i < 32 * 64; i += 256) {
-                const int k = i % 32, r = i / 32, wk = p.w_mn ? i / 64 : k, wr = p.w_mn ? i % 64 : r;
-                float v[4], x = 0.f, w = 0.f;
-                if (k0 + k < p.K && m0 + r < p.M) {
-                    decode4(p.x.q[(m0 + r) * p.x.ldq + k0 + k], true, v);
-                    x = v[0] * p.x.scale[((k0 + k) / BLOCK) * p.x.lds + m0 + r];
-                }
-                if (k0 + wk < p.K && n0 + wr < p.N) {
-                    const long n = n0 + wr, kk = k0 + wk;
-                    decode4(p.w.q[p.w_mn ? kk * p.w.ldq + n : n * p.w.ldq + kk], true, v);
-                    w = v[0] * p.w.scale[p.w_mn ? (n / BLOCK) * p.w.lds + kk / BLOCK
-                                                : (kk / BLOCK) * p.w.lds + n / BLOCK];
-                }
-                xs[k][r] = x;
-                ws[wk][wr] = w;
-            }
-            __syncthreads();
-            for (int k = 0; k < 32; ++k)
-                for (int i = 0; i < 4; ++i)
-                    for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(xs[k][ty + 16 * i], ws[k][tx + 16 * j], acc[i][j]);
-            __syncthreads();
-        }
+constexpr int BM = 128, BK = 128;
+constexpr int A_BYTES = BM * BK;
+constexpr int NTHREADS = 384;  // four warps that feed, eight that add
+constexpr int ADDERS = 8;
+constexpr int EPI_LD = 36;     // floats per staged row of 32: 16-byte accesses of 8 lanes hit all banks
+constexpr int EPI_BYTES = 32 * EPI_LD * 4;  // per adding warp
+
+template <int BN>
+struct Shape {
+    static constexpr int B_BYTES = BN * BK;
+    static constexpr int STAGE = A_BYTES + B_BYTES;
+    static constexpr int STAGES = BN == 256 ? 3 : 5;
+    static constexpr int HALF = BN / 2;  // columns of an adding warp
+    static constexpr int EPI_OFF = STAGES * STAGE;
+    static constexpr int BAR_OFF = EPI_OFF + ADDERS * EPI_BYTES;
+    static constexpr int SMEM = BAR_OFF + 8 * (2 * STAGES + 5) + 16 + 1024 /*align*/;
+    static constexpr int TMEM = 2 * BN;
+};
+
+struct Maps {
+    CUtensorMap x, w;
+};
+
+struct Params {
+    long M, N, K;
+    int nk;           // k-blocks
+    long mt, nt;      // tiles
+    const float *sx, *sw;
+    long ldsx, ldsw;
+    const float* bias;
+    void* y;
+    int y_type, accumulate;
+    long ldy;
+    int vec;          // rows of y move four elements at a time
+    int* status;
+};
+
+__device__ __forceinline__ float old_value(const Params& p, long at) {
+    if (p.y_type == OP_F32) return static_cast<const float*>(p.y)[at];
+    if (p.y_type == OP_F16) return to_f32(static_cast<const f16*>(p.y)[at]);
+    return to_f32(static_cast<const __nv_bfloat16*>(p.y)[at]);
+}
+__device__ __forceinline__ void put_value(const Params& p, long at, float v) {
+    if (p.y_type == OP_F32) static_cast<float*>(p.y)[at] = v;
+    else if (p.y_type == OP_F16) static_cast<f16*>(p.y)[at] = from_f32<f16>(v);
+    else static_cast<__nv_bfloat16*>(p.y)[at] = from_f32<__nv_bfloat16>(v);
+}
+
+// four columns n .. n + 3 of row m: bias, old value, one rounding
+__device__ __forceinline__ void put4(const Params& p, long m, long n, float4 f) {
+    float v[4] = {f.x, f.y, f.z, f.w};
+    const long at = m * p.ldy + n;
+    const int left = p.N - n < 4 ? (int)(p.N - n) : 4;
+    if (p.bias)
+#pragma unroll
         for (int i = 0; i < 4; ++i)
-            for (int j = 0; j < 4; ++j) {
-                const long m = m0 + ty + 16 * i, n = n0 + tx + 16 * j;
-                if (m >= p.M || n >= p.N) continue;
-                const long at = m * p.y.ld + n;
-                const float v = acc[i][j] + (p.bias ? p.bias[n] : 0.f);
-                void* y = const_cast<void*>(p.y.p);
-                if (p.y.type == OP_F32) {
-                    float* o = static_cast<float*>(y) + at;
-                    *o = p.accumulate ? *o + v : v;
-                } else if (p.y.type == OP_F16) {
-                    f16* o = static_cast<f16*>(y) + at;
-                    *o = from_f32<f16>(p.accumulate ? to_f32(*o) + v : v);
-                } else {
-                    __nv_bfloat16* o = static_cast<__nv_bfloat16*>(y) + at;
-                    *o = from_f32<__nv_bfloat16>(p.accumulate ? to_f32(*o) + v : v);
+            if (i < left) v[i] += p.bias[n + i];
+    if (p.vec && left == 4) {
+        if (p.accumulate) {
+            float o[4];
+            load4_as<true>(p.y, p.y_type, at, 4, 0, o);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] += o[i];
+        }
+        store4_as<true>(p.y, p.y_type, at, 4, 0, v);
+        return;
+    }
+    for (int i = 0; i < left; ++i) put_value(p, at + i, p.accumulate ? old_value(p, at + i) + v[i] : v[i]);
+}
+
+template <int BN, bool MN>
+__global__ void __launch_bounds__(NTHREADS, 1) gemm_f8_kernel(const __grid_constant__ Maps maps, const Params p) {
+    typedef Shape<BN> S;
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw);
+    const uint32_t base = (raw + 1023) & ~1023u;
+    unsigned char* smem = smem_raw + (base - raw);
+    const uint32_t bars = base + S::BAR_OFF;
+    auto full_bar = [&](int s) { return bars + 8 * s; };
+    auto empty_bar = [&](int s) { return bars + 8 * (S::STAGES + s); };
+    auto tfull = [&](int b) { return bars + 8 * (2 * S::STAGES + b); };
+    auto tempty = [&](int b) { return bars + 8 * (2 * S::STAGES + 2 + b); };
+    const uint32_t drained = bars + 8 * (2 * S::STAGES + 4);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::BAR_OFF + 8 * (2 * S::STAGES + 5));
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        prefetch_tmap(&maps.x);
+        prefetch_tmap(&maps.w);
+        for (int s = 0; s < S::STAGES; ++s) {
+            mbar_init(full_bar(s), 1);
+            mbar_init(empty_bar(s), 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(tfull(b), 1);
+            mbar_init(tempty(b), ADDERS);
+        }
+        mbar_init(drained, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                     "r"(S::TMEM));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = *tmem_slot;
+    const long tiles = p.mt * p.nt;
+
+    // Registers: the four feeding warps give theirs to the eight that hold the sums (launched with
+    // 168 each: 128 * 56 + 256 * 224 = 384 * 168).
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == 0 && lane == 0) {
+            // -------------------------------------------------------- TMA
+            int s = 0;
+            uint32_t ph = 0;
+            long issued = 0;
+            bool ok = true;
+            for (long tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
+                const int m0 = (int)(tile / p.nt * BM), n0 = (int)(tile % p.nt * BN);
+                for (int kb = 0; kb < p.nk; ++kb, ++issued) {
+                    if (!mbar_wait_inline(empty_bar(s), ph ^ 1, p.status, 31)) { ok = false; break; }
+                    const uint32_t sa = base + s * S::STAGE, sb = sa + A_BYTES;
+                    mbar_expect_tx(full_bar(s), S::STAGE);
+                    tma_load_2d(sa, &maps.x, kb * BK, m0, full_bar(s));
+                    if (MN) {  // [K][N]: a box of 128 (n) x 128 (k) per 128 columns
+#pragma unroll
+                        for (int h = 0; h < BN / 128; ++h)
+                            tma_load_2d(sb + h * 16384, &maps.w, n0 + 128 * h, kb * BK, full_bar(s));
+                    } else {
+                        tma_load_2d(sb, &maps.w, kb * BK, n0, full_bar(s));
+                    }
+                    if (++s == S::STAGES) { s = 0; ph ^= 1; }
                 }
             }
+            if (!ok)  // let what was issued land before the CTA ends
+                for (long j = 0; j < S::STAGES && j < issued; ++j) {
+                    const long i = issued - 1 - j;
+                    mbar_drain_inline(full_bar((int)(i % S::STAGES)), (uint32_t)((i / S::STAGES) & 1));
+                }
+        } else if (warp == 1 && lane == 0) {
+            // -------------------------------------------------------- MMA
+            // fp32 accumulator (bit 4), E4M3 operands (0), B's major, N >> 3, M >> 4
+            const uint32_t idesc = (1u << 4) | ((uint32_t)MN << 16) | ((uint32_t)(BN >> 3) << 17) |
+                                   ((uint32_t)(BM >> 4) << 24);
+            const uint64_t a_desc = smem_desc(base, 16, 1024);
+            const uint64_t b_desc = MN ? smem_desc(base + A_BYTES, 16384, 1024) : smem_desc(base + A_BYTES, 16, 1024);
+            constexpr uint32_t b_step = (MN ? 32 * 128 : 32) >> 4;  // 32 of k: rows of 128 bytes, or bytes of a row
+            int s = 0, b = 0;
+            uint32_t ph = 0, bph = 0;
+            bool ok = true;
+            for (long tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
+                for (int kb = 0; kb < p.nk; ++kb) {
+                    if (!mbar_wait_inline(tempty(b), bph ^ 1, p.status, 32) || !mbar_wait_inline(full_bar(s), ph, p.status, 33)) {
+                        ok = false;
+                        break;
+                    }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint64_t off = (uint64_t)((s * S::STAGE) >> 4);
+#pragma unroll
+                    for (int k = 0; k < BK / 32; ++k)
+                        mma_f8(tmem + b * BN, a_desc + off + 2 * k, b_desc + off + b_step * k, idesc, k > 0);
+                    mma_commit(empty_bar(s));
+                    mma_commit(tfull(b));
+                    if (++s == S::STAGES) { s = 0; ph ^= 1; }
+                    b ^= 1;
+                    if (b == 0) bph ^= 1;
+                }
+            }
+            if (!ok) {  // the MMAs in flight write TMEM: wait for them before it is freed
+                mma_commit(drained);
+                mbar_drain_inline(drained, 0);
+            }
+        }
+    } else {
+        // ------------------------------------------------------------ adding warps
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        const int quad = warp & 3, half = (warp - 4) >> 2;
+        const uint32_t tcol = tmem + ((uint32_t)(quad * 32) << 16) + half * S::HALF;
+        float* stage = reinterpret_cast<float*>(smem + S::EPI_OFF + (warp - 4) * EPI_BYTES);
+        int b = 0;
+        uint32_t bph = 0;
+        bool ok = true;
+        for (long tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
+            const long m0 = tile / p.nt * BM + quad * 32, n0 = tile % p.nt * BN + half * S::HALF;
+            const long m = m0 + lane, nb = n0 / 128;
+            const float* sx = p.sx + (m < p.M ? m : 0);
+            // W's scales: [k-block][n-block], or [n-block][k-block] of a weight stored [K][N]
+            const float* sw = p.sw + (n0 < p.N ? (MN ? nb * p.ldsw : nb) : 0);
+            const long wstep = MN ? 1 : p.ldsw;
+            uint64_t acc[S::HALF / 2];
+#pragma unroll
+            for (int i = 0; i < S::HALF / 2; ++i) acc[i] = 0;
+            float a = sx[0], w = sw[0];
+            for (int kb = 0; kb < p.nk; ++kb) {
+                const uint64_t sc = pack2(a * w);
+                if (kb + 1 < p.nk) {
+                    a = sx[(long)(kb + 1) * p.ldsx];
+                    w = sw[(long)(kb + 1) * wstep];
+                }
+                bool got = true;
+                if (lane == 0) got = mbar_wait_inline(tfull(b), bph, p.status, 34);
+                if (!__shfl_sync(FULL, got ? 1 : 0, 0)) { ok = false; break; }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                uint32_t r[2][16];
+                tmem_ld16_start(tcol + b * BN, r[0]);
+#pragma unroll
+                for (int c = 0; c < S::HALF / 16; ++c) {
+                    tmem_ld16_wait(r[c & 1]);
+                    if (c + 1 < S::HALF / 16) {
+                        tmem_ld16_start(tcol + b * BN + 16 * (c + 1), r[(c + 1) & 1]);
+                    } else {  // all of this warp's part is read: hand the buffer back
+                        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                        if (lane == 0) mbar_arrive(tempty(b));
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) fma2(acc[8 * c + i], r[c & 1][2 * i], r[c & 1][2 * i + 1], sc);
+                }
+                b ^= 1;
+                if (b == 0) bph ^= 1;
+            }
+            if (!ok) break;
+            // epilogue: 32 x 32 at a time, a row per lane in, four rows of 128 bytes per access out
+#pragma unroll
+            for (int c = 0; c < S::HALF / 32; ++c) {
+                if (n0 + 32 * c >= p.N) break;
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float2 u = unpack2(acc[16 * c + 2 * i]), v = unpack2(acc[16 * c + 2 * i + 1]);
+                    *reinterpret_cast<float4*>(stage + lane * EPI_LD + 4 * i) = make_float4(u.x, u.y, v.x, v.y);
+                }
+                __syncwarp();
+#pragma unroll 1
+                for (int i = 0; i < 8; ++i) {
+                    const int r = 4 * i + (lane >> 3);
+                    const long n = n0 + 32 * c + 4 * (lane & 7);
+                    const float4 f = *reinterpret_cast<const float4*>(stage + r * EPI_LD + 4 * (lane & 7));
+                    if (m0 + r < p.M && n < p.N) put4(p, m0 + r, n, f);
+                }
+            }
+        }
     }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (warp == 0)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::TMEM));
+}
+
+// ---------------------------------------------------------------------------------------
+constexpr int SM_WARPS = 4;   // k-blocks of a CTA go round its warps
+constexpr int SM_ROWS = 16;   // rows of W a CTA owns
+constexpr int SM_MAX_M = 16;
+
+__device__ __forceinline__ void mma_sync_e4m3(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};\n"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// 32 codes from k on (16-byte aligned); codes at or past K read as 0
+__device__ __forceinline__ void load32(const uint8_t* row, long k, long K, bool in, uint32_t r[8]) {
+    uint4 v[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+        if (in && k + 16 * h < K) v[h] = *reinterpret_cast<const uint4*>(row + k + 16 * h);
+    const uint32_t w[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = w[i];
+    if (k + 32 > K)  // the row's end: what follows it in memory is anyone's
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const long left = K - (k + 4 * i);
+            r[i] = left >= 4 ? r[i] : left > 0 ? r[i] & (0xffffffffu >> (32 - 8 * (int)left)) : 0u;
+        }
+}
+
+// MT groups of eight rows of X
+template <int MT>
+__global__ void __launch_bounds__(SM_WARPS * 32) gemm_f8_small_kernel(const uint8_t* x, long ldx, const uint8_t* w,
+                                                                      long ldw, const Params p) {
+    __shared__ float part[SM_WARPS][8 * MT][SM_ROWS + 1];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const long n0 = (long)blockIdx.x * SM_ROWS;
+    float acc[MT][4] = {};
+#pragma unroll 2
+    for (int kb = warp; kb < p.nk; kb += SM_WARPS) {
+        const long k = (long)kb * BK + 32 * t;
+        uint32_t a[2][8], b[MT][8];
+        load32(w + (n0 + g) * ldw, k, p.K, n0 + g < p.N, a[0]);
+        load32(w + (n0 + g + 8) * ldw, k, p.K, n0 + g + 8 < p.N, a[1]);
+        float s[MT][2];
+        const float sw = p.sw[(long)kb * p.ldsw + n0 / 128];
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {
+            load32(x + (8 * j + g) * ldx, k, p.K, 8 * j + g < p.M, b[j]);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int m = 8 * j + 2 * t + c;
+                s[j][c] = m < p.M ? sw * p.sx[(long)kb * p.ldsx + m] : 0.f;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {
+            float d[4] = {};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t f[4] = {a[0][2 * i], a[1][2 * i], a[0][2 * i + 1], a[1][2 * i + 1]};
+                mma_sync_e4m3(d, f, b[j][2 * i], b[j][2 * i + 1]);
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c) acc[j][c] = fmaf(d[c], s[j][c & 1], acc[j][c]);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < MT; ++j)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) part[warp][8 * j + 2 * t + (c & 1)][g + 8 * (c >> 1)] = acc[j][c];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 8 * MT * SM_ROWS; i += SM_WARPS * 32) {
+        const int m = i / SM_ROWS, r = i % SM_ROWS;
+        const long n = n0 + r;
+        if (m >= p.M || n >= p.N) continue;
+        float v = 0.f;
+#pragma unroll
+        for (int q = 0; q < SM_WARPS; ++q) v += part[q][m][r];
+        if (p.bias) v += p.bias[n];
+        const long at = m * p.ldy + n;
+        put_value(p, at, p.accumulate ? old_value(p, at) + v : v);
+    }
+}
+
+template <int BN, bool MN>
+void launch(const GemmF8& a, Params p, cudaStream_t s) {
+    typedef Shape<BN> S;
+    static DeviceOnce once;
+    once([] {
+        cudaFuncSetAttribute(gemm_f8_kernel<BN, MN>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+    });
+    Maps maps;
+    tc_make_map_u8(&maps.x, a.x.q, a.M, a.K, a.x.ldq, BK, BM);
+    if (MN) tc_make_map_u8(&maps.w, a.w.q, a.K, a.N, a.w.ldq, 128, BK);
+    else tc_make_map_u8(&maps.w, a.w.q, a.N, a.K, a.w.ldq, BK, BN);
+    p.mt = (a.M + BM - 1) / BM;
+    p.nt = (a.N + BN - 1) / BN;
+    const long tiles = p.mt * p.nt, sms = current_sm_count();
+    gemm_f8_kernel<BN, MN><<<(unsigned)(tiles < sms ? tiles : sms), NTHREADS, S::SMEM, s>>>(maps, p);
 }
 
 }  // namespace
 
 void gemm_f8(const GemmF8& a, cudaStream_t s) {
-    const long mt = (a.M + 63) / 64;
-    gemm_f8_kernel<<<dim3((unsigned)((a.N + 63) / 64), (unsigned)(mt < 65535 ? mt : 65535)), 256, 0, s>>>(a);
+    Params p;
+    p.M = a.M; p.N = a.N; p.K = a.K; p.nk = (int)((a.K + BK - 1) / BK);
+    p.sx = a.x.scale; p.sw = a.w.scale; p.ldsx = a.x.lds; p.ldsw = a.w.lds;
+    p.bias = a.bias; p.y = const_cast<void*>(a.y.p); p.y_type = a.y.type; p.accumulate = a.accumulate ? 1 : 0;
+    p.ldy = a.y.ld; p.vec = vec4(a.y) ? 1 : 0; p.status = a.status;
+    p.mt = p.nt = 0;
+    if (a.M <= SM_MAX_M && !a.w_mn) {
+        const unsigned ctas = (unsigned)((a.N + SM_ROWS - 1) / SM_ROWS);
+        if (a.M <= 8) gemm_f8_small_kernel<1><<<ctas, SM_WARPS * 32, 0, s>>>(a.x.q, a.x.ldq, a.w.q, a.w.ldq, p);
+        else gemm_f8_small_kernel<2><<<ctas, SM_WARPS * 32, 0, s>>>(a.x.q, a.x.ldq, a.w.q, a.w.ldq, p);
+        return;
+    }
+    // 256-wide tiles unless 128-wide ones finish in fewer column-rounds over the SMs
+    const long mt = (a.M + BM - 1) / BM, sms = current_sm_count();
+    auto cost = [&](long bn) { return (mt * ((a.N + bn - 1) / bn) + sms - 1) / sms * bn; };
+    if (cost(128) < cost(256)) a.w_mn ? launch<128, true>(a, p, s) : launch<128, false>(a, p, s);
+    else a.w_mn ? launch<256, true>(a, p, s) : launch<256, false>(a, p, s);
 }
 
 }  // namespace act

@@ -1362,6 +1362,19 @@ void tc_make_map_raw(CUtensorMap* map, const void* ptr, bool f16v, long rows, lo
     make_map_raw(map, ptr, f16v, rows, cols, ld, box_cols, box_rows);
 }
 
+void tc_make_map_u8(CUtensorMap* map, const void* ptr, long rows, long cols, long ld, int box_cols, int box_rows) {
+    if ((reinterpret_cast<uintptr_t>(ptr) & 15) || ld % 16)
+        throw std::runtime_error("tc_make_map_u8: operand not 16-byte aligned");
+    cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)ld};
+    cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
+    cuuint32_t estr[2] = {1, 1};
+    CUresult r = encode_fn()(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, estr,
+                             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) throw std::runtime_error("cuTensorMapEncodeTiled (bytes) failed: " + std::to_string((int)r));
+}
+
 void tc_make_map3(CUtensorMap* map, const f16* ptr, long clips, long rows, long cols, long ld, int box_cols,
                   int box_rows) {
     if ((reinterpret_cast<uintptr_t>(ptr) & 15) || (ld * 2) % 16)

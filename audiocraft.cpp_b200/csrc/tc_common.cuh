@@ -71,6 +71,26 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int* er
     return mbar_try(bar, parity) || mbar_wait_slow(bar, parity, err, code);
 }
 
+// The same wait without a call, for code whose warps took registers from others (setmaxnreg): a call
+// would have to save them all.
+__device__ __forceinline__ bool mbar_wait_inline(uint32_t bar, uint32_t parity, int* err, int code) {
+    if (mbar_try(bar, parity)) return true;
+    const unsigned long long t0 = globaltimer();
+    while (!mbar_try_sleep(bar, parity, 100000u)) {
+        if (globaltimer() - t0 > WAIT_NS) {
+            atomicCAS(err, 0, code);
+            return false;
+        }
+        if (*(volatile int*)err) return false;
+    }
+    return true;
+}
+__device__ __forceinline__ void mbar_drain_inline(uint32_t bar, uint32_t parity) {
+    const unsigned long long t0 = globaltimer();
+    while (!mbar_try_sleep(bar, parity, 20000u))
+        if (globaltimer() - t0 > 100000000ull) return;
+}
+
 // Wait for copies this thread issued to land before its CTA exits, after another wait failed:
 // bounded (limit_ns) but not cut short by the error word, which is already set by then.
 static __device__ __noinline__ void mbar_wait_drain(uint32_t bar, uint32_t parity,
@@ -156,6 +176,16 @@ __device__ __forceinline__ void mma_f16(uint32_t tmem_d, uint64_t adesc, uint64_
         ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate));
 }
 
+// 8-bit floating point operands (32 of the reduction per instruction)
+__device__ __forceinline__ void mma_f8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                       uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate));
+}
+
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
                  : "memory");
@@ -171,6 +201,39 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
           "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(taddr));
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+// 16 columns without the wait, and the wait that owns the registers: nothing that reads them can
+// be moved above it.
+__device__ __forceinline__ void tmem_ld16_start(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld16_wait(uint32_t* r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+        : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+          "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+        :: "memory");
+}
+
+// acc (two fp32 in one 64-bit register) += {lo, hi} * {s, s}: two fused multiply-adds, one instruction
+__device__ __forceinline__ void fma2(uint64_t& acc, uint32_t lo, uint32_t hi, uint64_t s2) {
+    uint64_t t;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(t) : "r"(lo), "r"(hi));
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(t), "l"(s2));
+}
+__device__ __forceinline__ uint64_t pack2(float v) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %1};" : "=l"(r) : "r"(__float_as_uint(v)));
+    return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+    uint32_t a, b;
+    asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(v));
+    return make_float2(__uint_as_float(a), __uint_as_float(b));
 }
 
 // ---------------------------------------------------------------------------------------
@@ -265,6 +328,8 @@ void tc_make_map(CUtensorMap* map, const f16* ptr, long rows, long cols, long ld
 // scales), [rows][cols] with row stride ld elements, box {box_cols, box_rows}.
 void tc_make_map_raw(CUtensorMap* map, const void* ptr, bool f16v, long rows, long cols, long ld, int box_cols,
                      int box_rows);
+// 2-D tensor of bytes [rows][cols], row stride ld; box {box_cols <= 128, box_rows}, 128-byte swizzle.
+void tc_make_map_u8(CUtensorMap* map, const void* ptr, long rows, long cols, long ld, int box_cols, int box_rows);
 // 3-D f16 tensor [clips][rows][cols] (row stride ld elements, clip stride rows * ld): a box
 // {box_cols, box_rows, 1} never crosses into the next clip (rows past `rows` read as zero).
 void tc_make_map3(CUtensorMap* map, const f16* ptr, long clips, long rows, long cols, long ld, int box_cols,
