@@ -1,60 +1,483 @@
 // rank_ckpt8.cu -- the rank product that reads an 8-bit checkpoint: C[j][c] (+)= alpha * sum over
 // rows t of U[t][j] * X[t][c], the lora_A gradient from a kept input.
 //
-// A CTA owns 64 columns of C and all nb <= 64 of its rows; X is decoded on its way into shared
-// memory, sums are fp32 in registers.
+// X is read once and the work per byte is small, so the kernel is bound by HBM as long as turning
+// codes into tensor-core operands keeps up.  A CTA owns 128 or 256 columns of X (the rows of the MMA)
+// and a slice of the rows t (the reduction), in blocks of 64:
+//   warp 0     TMA: raw codes into a ring of 64-row blocks
+//   warps 8-15 codes * scale -> bf16 (exact: 4 or 7 significant bits times a power of two) in the
+//              128-byte-swizzled MN-major layout; the block's rows of U, cut into bf16 pieces that add
+//              up to it exactly (one for bf16, two for f16, three for fp32): both operands of the
+//              MMA have to be bf16, and the product keeps all of U
+//   warp 1     tcgen05 MMAs: one accumulator for the leading pieces, one for the others
+//   warps 4-7  the sums: the tensor cores cut each addition into the accumulator off below its last bit
+//              (measured: a relative 2^-24 downwards per 16 rows, 5e-6 over 4000 rows), so the
+//              leading accumulator is emptied into fp32 registers every 256 rows, two of them in turn;
+//              the others are at least 2^-8 smaller and are added once, at the end
+// The slices of a column tile form a cluster and add their sums in order through distributed
+// shared memory: no atomics, the same bits every time.
+#include <cuda.h>
+
 #include "ckpt8.cuh"
+#include "tc_common.cuh"
 
 namespace act {
 
 namespace {
 
 using namespace c8;
+using namespace tc;
 
-__global__ void __launch_bounds__(256) rank_kernel(const RankCkpt8 p) {
-    __shared__ float us[32][65], xs[32][65];
-    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    const long c0 = (long)blockIdx.x * 64;
-    float acc[4][4] = {};
-    for (long t0 = 0; t0 < p.rows; t0 += 32) {
-        for (int i = threadIdx.x; i < 32 * 64; i += 256) {
-            const int r = i / 64, c = i % 64;
-            const long t = t0 + r;
-            float u = 0.f, x = 0.f;
-            if (t < p.rows && c < p.nb) {
-                const long at = t * p.u.ld + c;
-                u = p.u.type == OP_F32 ? static_cast<const float*>(p.u.p)[at]
-                    : p.u.type == OP_F16 ? to_f32(static_cast<const f16*>(p.u.p)[at])
-                                         : to_f32(static_cast<const __nv_bfloat16*>(p.u.p)[at]);
-            }
-            if (t < p.rows && c0 + c < p.cols) {
-                float v[4];
-                decode4(p.x.q[t * p.x.ldq + c0 + c], p.x.e4m3, v);
-                x = v[0] * p.x.scale[((c0 + c) / BLOCK) * p.x.lds + t];
-            }
-            us[r][c] = u;
-            xs[r][c] = x;
-        }
-        __syncthreads();
-        for (int r = 0; r < 32; ++r)
-            for (int i = 0; i < 4; ++i)
-                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(us[r][ty + 16 * i], xs[r][tx + 16 * j], acc[i][j]);
-        __syncthreads();
+constexpr int RK = 64;                   // rows t of a block
+constexpr int RGROUP = 4;                // blocks between two emptyings of the leading accumulator
+constexpr int RTHREADS = 512;
+constexpr int RCONV = 8;                 // converting warps; each takes 8 rows of a block
+constexpr int RA_BYTES = 128 * RK * 2;   // bf16 operand of 128 columns
+constexpr int RB_BOX = RK * 64 * 2;      // 64 columns of pieces
+constexpr int RMAX_SPLIT = 8;            // portable cluster size
+
+// T: tiles of 128 columns per CTA
+template <int T>
+struct RShape {
+    static constexpr int RAW = T * 128 * RK;
+    static constexpr int RAWS = T == 2 ? 6 : 8;
+    static constexpr int OP = T * RA_BYTES + 3 * RB_BOX;
+    static constexpr int OPS = T == 2 ? 2 : 3;
+    static constexpr int RAW_OFF = OPS * OP;
+    static constexpr int BAR_OFF = RAW_OFF + RAWS * RAW;
+    static constexpr int NBARS = 2 * RAWS + 2 * OPS + 6;
+    static constexpr int SMEM = BAR_OFF + 8 * NBARS + 16 + 1024 /*align*/;
+    static constexpr int TMEM = 256 * T;     // leading: 2 x T x 64 columns, others: T x 128
+    static constexpr int OTHER = 128 * T;    // first column of the others
+    static constexpr int LD = T * 128 + 4;   // floats of a row of the sums in shared memory
+    static_assert(64 * LD * 4 <= RAW_OFF, "the sums take the operand ring's place");
+};
+
+struct RParams {
+    int rows, nk, nb, nbp;  // nbp: nb rounded up to 16
+    long cols;
+    const void* u;
+    int u_type, u_vec, pieces;
+    long ldu;
+    const float* scale;
+    long lds;
+    int e4m3;
+    float alpha;
+    float* c;
+    long ldc;
+    int c_vec, accumulate, splits;
+    int* status;
+};
+
+struct RMaps {
+    CUtensorMap x;
+};
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+
+// four codes times s -> four bf16
+__device__ __forceinline__ uint2 codes_to_bf16(uint32_t w, float s, bool e4m3) {
+    if (e4m3) {
+        float v[4];
+        decode4(w, true, v);
+        return make_uint2(pack_bf16(v[0] * s, v[1] * s), pack_bf16(v[2] * s, v[3] * s));
     }
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) {
-            const int r = ty + 16 * i;
-            const long c = c0 + tx + 16 * j;
-            if (r >= p.nb || c >= p.cols) continue;
-            float* o = p.c + r * p.ldc + c;
-            *o = p.accumulate ? *o + p.alpha * acc[i][j] : p.alpha * acc[i][j];
+    // q + 128 in the low byte of 2^23, less 2^23 + 128, times s: exact throughout
+    const uint32_t x = w ^ 0x80808080u;
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = (__uint_as_float(__byte_perm(x, 0x4b000000u, 0x7650 + i)) - 8388736.0f) * s;
+    if ((x - 0x01010101u) & ~x & 0x80808080u)  // a zero byte: the code -128 (a borrow may flag the byte above)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (((x >> (8 * i)) & 0xffu) == 0) v[i] = __int_as_float(0x7fc00000);
+    return make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+}
+
+// eight values of row t of U from column j on; missing rows and columns are 0
+__device__ __forceinline__ void load_u(const RParams& p, long t, int j, float v[8]) {
+    const bool in = t < p.rows;
+    const long at = t * p.ldu + j;
+    if (in && p.u_vec && j + 8 <= p.nb) {
+        if (p.u_type == OP_F32) {
+            const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(p.u) + at);
+            const float4 b = *reinterpret_cast<const float4*>(static_cast<const float*>(p.u) + at + 4);
+            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+            v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        } else {
+            const uint2 a = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.u) + at);
+            const uint2 b = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.u) + at + 4);
+            const uint32_t w[4] = {a.x, a.y, b.x, b.y};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 f = p.u_type == OP_F16 ? unpack_f16(w[i]) : make_float2(bf16_lo(w[i]), bf16_hi(w[i]));
+                v[2 * i] = f.x;
+                v[2 * i + 1] = f.y;
+            }
         }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        v[i] = 0.f;
+        if (in && j + i < p.nb)
+            v[i] = p.u_type == OP_F32   ? static_cast<const float*>(p.u)[at + i]
+                   : p.u_type == OP_F16 ? to_f32(static_cast<const f16*>(p.u)[at + i])
+                                        : to_f32(static_cast<const __nv_bfloat16*>(p.u)[at + i]);
+    }
+}
+
+// The next bf16 piece of v is its upper half-word (cut off, not rounded: three pieces hold all 24 bits
+// and none can overflow); what is left of v is exact.  An infinity is all in its first piece.
+__device__ __forceinline__ float left_of(float v) {
+    return abs_bits(v) == 0x7f800000u ? 0.f : v - __uint_as_float(__float_as_uint(v) & 0xffff0000u);
+}
+
+template <int T>
+__global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant__ RMaps maps, const RParams p) {
+    typedef RShape<T> S;
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw);
+    const uint32_t base = (raw + 1023) & ~1023u;
+    unsigned char* smem = smem_raw + (base - raw);
+    const uint32_t bars = base + S::BAR_OFF;
+    auto raw_full = [&](int s) { return bars + 8 * s; };
+    auto raw_empty = [&](int s) { return bars + 8 * (S::RAWS + s); };
+    auto op_full = [&](int s) { return bars + 8 * (2 * S::RAWS + s); };
+    auto op_empty = [&](int s) { return bars + 8 * (2 * S::RAWS + S::OPS + s); };
+    auto lead_full = [&](int b) { return bars + 8 * (2 * S::RAWS + 2 * S::OPS + b); };
+    auto lead_empty = [&](int b) { return bars + 8 * (2 * S::RAWS + 2 * S::OPS + 2 + b); };
+    const uint32_t all_done = bars + 8 * (2 * S::RAWS + 2 * S::OPS + 4);
+    const uint32_t drained = all_done + 8;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::BAR_OFF + 8 * S::NBARS);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const long c0 = (long)blockIdx.x * (T * 128);
+    const int split = blockIdx.y;
+    const int kb0 = (int)((long)p.nk * split / p.splits), kb1 = (int)((long)p.nk * (split + 1) / p.splits);
+
+    if (threadIdx.x == 0) {
+        prefetch_tmap(&maps.x);
+        for (int s = 0; s < S::RAWS; ++s) {
+            mbar_init(raw_full(s), 1);
+            mbar_init(raw_empty(s), RCONV);
+        }
+        for (int s = 0; s < S::OPS; ++s) {
+            mbar_init(op_full(s), RCONV);
+            mbar_init(op_empty(s), 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(lead_full(b), 1);
+            mbar_init(lead_empty(b), 4);
+        }
+        mbar_init(all_done, 1);
+        mbar_init(drained, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                     "r"(S::TMEM));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = *tmem_slot;
+
+    // Launched with 128 registers a thread: 48 + 192 + 2 * 136 = 4 * 128.
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+        if (warp == 0 && lane == 0) {
+            // -------------------------------------------------------- TMA
+            int s = 0, issued = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            for (int kb = kb0; kb < kb1; ++kb, ++issued) {
+                if (!mbar_wait_inline(raw_empty(s), ph ^ 1, p.status, 41)) { ok = false; break; }
+                mbar_expect_tx(raw_full(s), S::RAW);
+                tma_load_2d(base + S::RAW_OFF + s * S::RAW, &maps.x, (int)c0, kb * RK, raw_full(s));
+                if (++s == S::RAWS) { s = 0; ph ^= 1; }
+            }
+            if (!ok)  // let what was issued land before the CTA ends
+                for (int j = 0; j < S::RAWS && j < issued; ++j) {
+                    const int i = issued - 1 - j;
+                    mbar_drain_inline(raw_full(i % S::RAWS), (uint32_t)((i / S::RAWS) & 1));
+                }
+        } else if (warp == 1 && lane == 0) {
+            // -------------------------------------------------------- MMA
+            // fp32 accumulator, bf16 operands (1), both MN-major, N >> 3, M >> 4
+            const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (1u << 16) | (8u << 24);
+            const uint32_t lead_desc = idesc | ((uint32_t)(p.nbp >> 3) << 17);
+            const uint32_t other_desc = idesc | ((uint32_t)(((p.pieces - 1) * p.nbp) >> 3) << 17);
+            const uint64_t a_desc = smem_desc(base, 8192, 1024);
+            const uint64_t b_desc = smem_desc(base + T * RA_BYTES, 8192, 1024);
+            constexpr uint32_t step = 2048 >> 4;  // 16 rows of 128 bytes
+            int s = 0, b = 0;
+            uint32_t ph = 0, bph = 0;
+            bool ok = true;
+            for (int kb = kb0; kb < kb1; ++kb) {
+                const int in_group = (kb - kb0) % RGROUP;
+                if (in_group == 0 && !mbar_wait_inline(lead_empty(b), bph ^ 1, p.status, 42)) { ok = false; break; }
+                if (!mbar_wait_inline(op_full(s), ph, p.status, 43)) { ok = false; break; }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint64_t off = (uint64_t)((s * S::OP) >> 4);
+#pragma unroll
+                for (int t = 0; t < T; ++t) {
+                    const uint64_t a = a_desc + off + (t * RA_BYTES >> 4), bb = b_desc + off;
+#pragma unroll
+                    for (int k = 0; k < RK / 16; ++k)
+                        mma_f16(tmem + (b * T + t) * 64, a + step * k, bb + step * k, lead_desc,
+                                (in_group > 0 || k > 0) ? 1u : 0u);
+                    if (p.pieces > 1)
+#pragma unroll
+                        for (int k = 0; k < RK / 16; ++k)
+                            mma_f16(tmem + S::OTHER + t * 128, a + step * k, bb + (RB_BOX >> 4) + step * k, other_desc,
+                                    (kb > kb0 || k > 0) ? 1u : 0u);
+                }
+                mma_commit(op_empty(s));
+                if (++s == S::OPS) { s = 0; ph ^= 1; }
+                if (in_group == RGROUP - 1 || kb == kb1 - 1) {
+                    mma_commit(lead_full(b));
+                    b ^= 1;
+                    if (b == 0) bph ^= 1;
+                }
+            }
+            if (ok) {
+                mma_commit(all_done);
+            } else {  // the MMAs in flight write TMEM: wait for them before it is freed
+                mma_commit(drained);
+                mbar_drain_inline(drained, 0);
+            }
+        }
+    } else if (warp < 8) {
+        // ------------------------------------------------------------ sums
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+        const int quad = warp & 3;
+        const uint32_t tl = tmem + ((uint32_t)(quad * 32) << 16);
+        float sum[T][64];
+#pragma unroll
+        for (int t = 0; t < T; ++t)
+#pragma unroll
+            for (int i = 0; i < 64; ++i) sum[t][i] = 0.f;
+        int b = 0;
+        uint32_t bph = 0;
+        bool ok = true;
+        for (int kb = kb0; kb < kb1; kb += RGROUP) {
+            bool got = true;
+            if (lane == 0) got = mbar_wait_inline(lead_full(b), bph, p.status, 44);
+            if (!__shfl_sync(FULL, got ? 1 : 0, 0)) { ok = false; break; }
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+            for (int t = 0; t < T; ++t)
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (16 * c < p.nbp) {
+                        uint32_t r[16];
+                        tmem_ld16_start(tl + (b * T + t) * 64 + 16 * c, r);
+                        tmem_ld16_wait(r);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) sum[t][16 * c + i] += __uint_as_float(r[i]);
+                    }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            if (lane == 0) mbar_arrive(lead_empty(b));
+            b ^= 1;
+            if (b == 0) bph ^= 1;
+        }
+        if (ok) {  // every MMA is done: the others' accumulators are whole, the operand ring is free
+            bool got = true;
+            if (lane == 0) got = mbar_wait_inline(all_done, 0, p.status, 45);
+            ok = __shfl_sync(FULL, got ? 1 : 0, 0) != 0;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        }
+        if (ok) {
+            float* part = reinterpret_cast<float*>(smem);
+#pragma unroll
+            for (int t = 0; t < T; ++t) {
+                for (int q = p.pieces - 1; q > 0; --q)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        if (16 * c < p.nbp) {
+                            uint32_t r[16];
+                            tmem_ld16_start(tl + S::OTHER + t * 128 + (q - 1) * p.nbp + 16 * c, r);
+                            tmem_ld16_wait(r);
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) sum[t][16 * c + i] += __uint_as_float(r[i]);
+                        }
+#pragma unroll
+                for (int i = 0; i < 64; ++i)
+                    if (i < p.nb) part[i * S::LD + t * 128 + quad * 32 + lane] = sum[t][i];
+            }
+        }
+    } else {
+        // ------------------------------------------------------------ codes and U to bf16
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
+        constexpr int LPR = 16 * T;        // lanes of a row (8 codes each)
+        constexpr int RPP = 32 / LPR;      // rows of a pass
+        const int cw = warp - 8;           // rows 8 cw .. 8 cw + 7 of each block
+        const int units = p.nbp >> 3;      // 8-column units of a row of U
+        const int cl = lane % LPR, tile = cl >> 4, box = (cl >> 3) & 1, unit = cl & 7;
+        const long fb = c0 / BLOCK + (lane >> 3);  // whose scale lanes 0 .. 8 T - 1 fetch
+        const bool fetch = lane < 8 * T && fb * BLOCK < p.cols;
+        float un[2][8], sn = 0.f;
+        auto prefetch = [&](int kb) {
+            const long t0 = (long)kb * RK + 8 * cw;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int q = lane + 32 * i;
+                if (q < 8 * units) load_u(p, t0 + q / units, q % units * 8, un[i]);
+            }
+            const long t = t0 + (lane & 7);
+            sn = fetch && t < p.rows ? p.scale[fb * p.lds + t] : 0.f;
+        };
+        if (kb0 < kb1) prefetch(kb0);
+        int s = 0, o = 0;
+        uint32_t ph = 0, oph = 0;
+        for (int kb = kb0; kb < kb1; ++kb) {
+            float u[2][8];
+            const float sc = sn;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) u[i][j] = un[i][j];
+            if (kb + 1 < kb1) prefetch(kb + 1);
+            bool got = true;
+            if (lane == 0)
+                got = mbar_wait_inline(op_empty(o), oph ^ 1, p.status, 46) &&
+                      mbar_wait_inline(raw_full(s), ph, p.status, 47);
+            if (!__shfl_sync(FULL, got ? 1 : 0, 0)) break;
+            unsigned char* op = smem + o * S::OP;
+            const unsigned char* rw = smem + S::RAW_OFF + s * S::RAW;
+            uint2 w[8 / RPP];
+#pragma unroll
+            for (int i = 0; i < 8 / RPP; ++i)
+                w[i] = *reinterpret_cast<const uint2*>(rw + (8 * cw + i * RPP + lane / LPR) * (T * 128) + 8 * cl);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(raw_empty(s));
+#pragma unroll
+            for (int i = 0; i < 8 / RPP; ++i) {
+                const int r = i * RPP + lane / LPR;
+                const float sr = __shfl_sync(FULL, sc, 8 * tile + r);
+                const uint2 a = codes_to_bf16(w[i].x, sr, p.e4m3), b = codes_to_bf16(w[i].y, sr, p.e4m3);
+                *reinterpret_cast<uint4*>(op + tile * RA_BYTES + box * 8192 + q8_sw128(8 * cw + r, unit)) =
+                    make_uint4(a.x, a.y, b.x, b.y);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int q = lane + 32 * i;
+                if (q >= 8 * units) break;
+                const int r = 8 * cw + q / units, j8 = q % units;
+                for (int piece = 0; piece < p.pieces; ++piece) {
+                    uint32_t h[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        h[j] = __byte_perm(__float_as_uint(u[i][2 * j]), __float_as_uint(u[i][2 * j + 1]), 0x7632);
+                        u[i][2 * j] = left_of(u[i][2 * j]);
+                        u[i][2 * j + 1] = left_of(u[i][2 * j + 1]);
+                    }
+                    // the leading pieces fill the first box, the others the next two, end to end
+                    const int col8 = piece == 0 ? j8 : 8 + (piece - 1) * units + j8;
+                    *reinterpret_cast<uint4*>(op + T * RA_BYTES + (col8 >> 3) * RB_BOX + q8_sw128(r, col8 & 7)) =
+                        make_uint4(h[0], h[1], h[2], h[3]);
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(op_full(o));
+            if (++s == S::RAWS) { s = 0; ph ^= 1; }
+            if (++o == S::OPS) { o = 0; oph ^= 1; }
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (warp == 0)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::TMEM));
+    // every thread of every CTA of the cluster passes both barriers
+    if (p.splits > 1) cluster_sync_all();
+    const uint32_t part = base;
+    const int rank = p.splits > 1 ? (int)cluster_ctarank() : 0;
+    constexpr int Q = T * 32;  // float4 of a row
+    const int items = p.nb * Q, i0 = (int)((long)items * rank / p.splits),
+              i1 = (int)((long)items * (rank + 1) / p.splits);
+    for (int i = i0 + threadIdx.x; i < i1; i += RTHREADS) {
+        const int j = i / Q, f = i % Q * 4;
+        const long c = c0 + f;
+        if (c >= p.cols) continue;
+        const uint32_t at = part + (uint32_t)(j * S::LD + f) * 4;
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int q = 0; q < p.splits; ++q) {  // slice order: the same sum whoever finished first
+            const float4 d = ld_dsmem_f4(p.splits > 1 ? map_cta(at, (uint32_t)q) : at);
+            v[0] += d.x; v[1] += d.y; v[2] += d.z; v[3] += d.w;
+        }
+        float* out = p.c + j * p.ldc + c;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] *= p.alpha;
+        if (p.c_vec && c + 4 <= p.cols) {
+            float4 w = make_float4(v[0], v[1], v[2], v[3]);
+            if (p.accumulate) {
+                const float4 old = *reinterpret_cast<const float4*>(out);
+                w.x += old.x; w.y += old.y; w.z += old.z; w.w += old.w;
+            }
+            *reinterpret_cast<float4*>(out) = w;
+        } else {
+            for (int k = 0; k < 4 && c + k < p.cols; ++k) out[k] = p.accumulate ? out[k] + v[k] : v[k];
+        }
+    }
+    if (p.splits > 1) cluster_sync_all();  // peers keep their sums until every reader is done
+}
+
+template <int T>
+void launch(const RankCkpt8& a, RParams p, cudaStream_t s) {
+    typedef RShape<T> S;
+    static DeviceOnce once;
+    once([] { cudaFuncSetAttribute(rank_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM); });
+    const long tiles = (a.cols + T * 128 - 1) / (T * 128);
+    long splits = current_sm_count() / tiles;
+    if (splits > RMAX_SPLIT) splits = RMAX_SPLIT;
+    if (splits > p.nk) splits = p.nk;
+    if (splits < 1) splits = 1;
+    p.splits = (int)splits;
+    RMaps maps;
+    tc_make_map_raw(&maps.x, a.x.q, false, a.rows, a.cols, a.x.ldq, T * 128, RK);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)tiles, (unsigned)splits, 1);
+    cfg.blockDim = dim3(RTHREADS, 1, 1);
+    cfg.dynamicSmemBytes = S::SMEM;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1;
+    attr[0].val.clusterDim.y = (unsigned)splits;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, rank_kernel<T>, maps, p);
 }
 
 }  // namespace
 
 void rank_ckpt8(const RankCkpt8& a, cudaStream_t s) {
-    rank_kernel<<<(unsigned)((a.cols + 63) / 64), 256, 0, s>>>(a);
+    if (!a.rows) {
+        cudaMemset2DAsync(a.c, a.ldc * sizeof(float), 0, a.cols * sizeof(float), a.nb, s);
+        return;
+    }
+    RParams p;
+    p.rows = (int)a.rows; p.nk = (int)((a.rows + RK - 1) / RK); p.nb = a.nb; p.nbp = (a.nb + 15) / 16 * 16;
+    p.cols = a.cols;
+    p.u = a.u.p; p.u_type = a.u.type; p.u_vec = vec4(a.u) ? 1 : 0; p.ldu = a.u.ld;
+    p.pieces = a.u.type == OP_F32 ? 3 : a.u.type == OP_F16 ? 2 : 1;
+    p.scale = a.x.scale; p.lds = a.x.lds; p.e4m3 = a.x.e4m3 ? 1 : 0; p.alpha = a.alpha;
+    p.c = a.c; p.ldc = a.ldc; p.c_vec = vec4(a.c) && a.ldc % 4 == 0 ? 1 : 0; p.accumulate = a.accumulate ? 1 : 0;
+    p.splits = 1; p.status = a.status;
+    // 256 columns a CTA halve the work on U per code, where that still leaves CTAs for most SMs
+    const long wide = (a.cols + 255) / 256;
+    if (wide * RMAX_SPLIT >= current_sm_count()) launch<2>(a, p, s);
+    else launch<1>(a, p, s);
 }
 
 }  // namespace act
