@@ -5,7 +5,7 @@
 // codes into tensor-core operands keeps up.  A CTA owns 128 or 256 columns of X (the rows of the MMA)
 // and a slice of the rows t (the reduction), in blocks of 64:
 //   warp 0     TMA: raw codes into a ring of 64-row blocks
-//   warps 8-15 codes * scale -> bf16 (exact: 4 or 7 significant bits times a power of two) in the
+//   warps 8-23 codes * scale -> bf16 (exact: 4 or 7 significant bits times a power of two) in the
 //              128-byte-swizzled MN-major layout; the block's rows of U, cut into bf16 pieces that add
 //              up to it exactly (one for bf16, two for f16, three for fp32): both operands of the
 //              MMA have to be bf16, and the product keeps all of U
@@ -17,6 +17,8 @@
 // The slices of a column tile form a cluster and add their sums in order through distributed
 // shared memory: no atomics, the same bits every time.
 #include <cuda.h>
+
+#include <atomic>
 
 #include "ckpt8.cuh"
 #include "tc_common.cuh"
@@ -30,8 +32,10 @@ using namespace tc;
 
 constexpr int RK = 64;                   // rows t of a block
 constexpr int RGROUP = 4;                // blocks between two emptyings of the leading accumulator
-constexpr int RTHREADS = 512;
-constexpr int RCONV = 8;                 // converting warps; each takes 8 rows of a block
+constexpr int RCONV = 16;                // converting warps
+constexpr int RAHEAD = 8;
+constexpr int RROWS = RK / RCONV;        // rows of a block each takes
+constexpr int RTHREADS = (8 + RCONV) * 32;
 constexpr int RA_BYTES = 128 * RK * 2;   // bf16 operand of 128 columns
 constexpr int RB_BOX = RK * 64 * 2;      // 64 columns of pieces
 constexpr int RMAX_SPLIT = 8;            // portable cluster size
@@ -61,7 +65,6 @@ struct RParams {
     long ldu;
     const float* scale;
     long lds;
-    int e4m3;
     float alpha;
     float* c;
     long ldc;
@@ -80,23 +83,59 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 __device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
-// four codes times s -> four bf16
-__device__ __forceinline__ uint2 codes_to_bf16(uint32_t w, float s, bool e4m3) {
-    if (e4m3) {
-        float v[4];
-        decode4(w, true, v);
-        return make_uint2(pack_bf16(v[0] * s, v[1] * s), pack_bf16(v[2] * s, v[3] * s));
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(__float_as_uint(lo)), "r"(__float_as_uint(hi)));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint32_t pack_bf16(uint64_t v) {
+    const float2 f = unpack2(v);
+    return pack_bf16(f.x, f.y);
+}
+
+// eight codes times s -> eight bf16
+template <bool E4M3>
+__device__ __forceinline__ uint4 codes_to_bf16(uint2 w, float s) {
+    const uint64_t s2 = pack2(s);
+    uint32_t o[4];
+    if (E4M3) {
+        const uint32_t q[4] = {w.x & 0xffffu, w.x >> 16, w.y & 0xffffu, w.y >> 16};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __half2 h = __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)q[i], __NV_E4M3));
+            const float2 f = __half22float2(h);
+            o[i] = pack_bf16(mul2(pair(f.x, f.y), s2));
+        }
+        return make_uint4(o[0], o[1], o[2], o[3]);
     }
     // q + 128 in the low byte of 2^23, less 2^23 + 128, times s: exact throughout
-    const uint32_t x = w ^ 0x80808080u;
-    float v[4];
+    const uint32_t x[2] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u};
+    const uint64_t bias = pack2(-8388736.0f);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = (__uint_as_float(__byte_perm(x, 0x4b000000u, 0x7650 + i)) - 8388736.0f) * s;
-    if ((x - 0x01010101u) & ~x & 0x80808080u)  // a zero byte: the code -128 (a borrow may flag the byte above)
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t y = x[i >> 1];
+        const int b = 2 * (i & 1);
+        const float lo = __uint_as_float(__byte_perm(y, 0x4b000000u, 0x7650 + b));
+        const float hi = __uint_as_float(__byte_perm(y, 0x4b000000u, 0x7651 + b));
+        o[i] = pack_bf16(mul2(add2(pair(lo, hi), bias), s2));
+    }
+    // a zero byte of x is the code -128, NaN (a borrow may flag the byte above it too)
+    const uint32_t z = ((x[0] - 0x01010101u) & ~x[0]) | ((x[1] - 0x01010101u) & ~x[1]);
+    if (z & 0x80808080u)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (((x >> (8 * i)) & 0xffu) == 0) v[i] = __int_as_float(0x7fc00000);
-    return make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+        for (int i = 0; i < 8; ++i)
+            if (((x[i >> 2] >> (8 * (i & 3))) & 0xffu) == 0) o[i >> 1] |= 0x7fc0u << (16 * (i & 1));
+    return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
 // eight values of row t of U from column j on; missing rows and columns are 0
@@ -138,7 +177,7 @@ __device__ __forceinline__ float left_of(float v) {
     return abs_bits(v) == 0x7f800000u ? 0.f : v - __uint_as_float(__float_as_uint(v) & 0xffff0000u);
 }
 
-template <int T>
+template <int T, bool E4M3>
 __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant__ RMaps maps, const RParams p) {
     typedef RShape<T> S;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -189,9 +228,9 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *tmem_slot;
 
-    // Launched with 128 registers a thread: 48 + 192 + 2 * 136 = 4 * 128.
+    // Launched with 80 registers a thread: 40 + 152 + 4 * 72 = 6 * 80.
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
         if (warp == 0 && lane == 0) {
             // -------------------------------------------------------- TMA
             int s = 0, issued = 0;
@@ -256,7 +295,7 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
         }
     } else if (warp < 8) {
         // ------------------------------------------------------------ sums
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
         const int quad = warp & 3;
         const uint32_t tl = tmem + ((uint32_t)(quad * 32) << 16);
         float sum[T][64];
@@ -315,36 +354,44 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
         }
     } else {
         // ------------------------------------------------------------ codes and U to bf16
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         constexpr int LPR = 16 * T;        // lanes of a row (8 codes each)
         constexpr int RPP = 32 / LPR;      // rows of a pass
-        const int cw = warp - 8;           // rows 8 cw .. 8 cw + 7 of each block
-        const int units = p.nbp >> 3;      // 8-column units of a row of U
+        const int cw = warp - 8, r0 = RROWS * cw;  // rows r0 .. r0 + RROWS - 1 of each block
         const int cl = lane % LPR, tile = cl >> 4, box = (cl >> 3) & 1, unit = cl & 7;
-        const long fb = c0 / BLOCK + (lane >> 3);  // whose scale lanes 0 .. 8 T - 1 fetch
-        const bool fetch = lane < 8 * T && fb * BLOCK < p.cols;
-        float un[2][8], sn = 0.f;
+        // U: RROWS x nbp / 8 units of 8 columns, at most one a lane
+        const int units = p.nbp >> 3, ur = lane / units, uj = lane % units;
+        const bool has_u = ur < RROWS;
+        const long fb = c0 / BLOCK + lane / RROWS;  // whose scale lanes 0 .. RROWS T - 1 fetch
+        const bool fetch = lane < RROWS * T && fb * BLOCK < p.cols;
+        const float* scales = p.scale + (fetch ? fb * p.lds : 0) + lane % RROWS;
+        float un[8], sn = 0.f;
         auto prefetch = [&](int kb) {
-            const long t0 = (long)kb * RK + 8 * cw;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int q = lane + 32 * i;
-                if (q < 8 * units) load_u(p, t0 + q / units, q % units * 8, un[i]);
-            }
-            const long t = t0 + (lane & 7);
-            sn = fetch && t < p.rows ? p.scale[fb * p.lds + t] : 0.f;
+            const int t0 = kb * RK + r0;
+            if (has_u) load_u(p, t0 + ur, 8 * uj, un);
+            sn = fetch && t0 + lane % RROWS < p.rows ? scales[t0] : 0.f;
         };
+        // U and the scales come straight to registers one block ahead, which covers L2's latency but not
+        // HBM's: they are called into L2 RAHEAD blocks before that
+        const char* ubase = static_cast<const char*>(p.u);
+        const int usize = p.u_type == OP_F32 ? 4 : 2;
+        auto call = [&](int kb) {
+            const int t0 = kb * RK + r0;
+            if (has_u && t0 + ur < p.rows && 8 * uj < p.nb)
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(ubase + ((long)(t0 + ur) * p.ldu + 8 * uj) * usize));
+            if (fetch && t0 + lane % RROWS < p.rows) asm volatile("prefetch.global.L2 [%0];" ::"l"(scales + t0));
+        };
+        for (int kb = kb0; kb < kb0 + RAHEAD && kb < kb1; ++kb) call(kb);
         if (kb0 < kb1) prefetch(kb0);
         int s = 0, o = 0;
         uint32_t ph = 0, oph = 0;
         for (int kb = kb0; kb < kb1; ++kb) {
-            float u[2][8];
+            float u[8];
             const float sc = sn;
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) u[i][j] = un[i][j];
+            for (int j = 0; j < 8; ++j) u[j] = un[j];
             if (kb + 1 < kb1) prefetch(kb + 1);
+            if (kb + RAHEAD < kb1) call(kb + RAHEAD);
             bool got = true;
             if (lane == 0)
                 got = mbar_wait_inline(op_empty(o), oph ^ 1, p.status, 46) &&
@@ -352,36 +399,30 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
             if (!__shfl_sync(FULL, got ? 1 : 0, 0)) break;
             unsigned char* op = smem + o * S::OP;
             const unsigned char* rw = smem + S::RAW_OFF + s * S::RAW;
-            uint2 w[8 / RPP];
+            uint2 w[RROWS / RPP];
 #pragma unroll
-            for (int i = 0; i < 8 / RPP; ++i)
-                w[i] = *reinterpret_cast<const uint2*>(rw + (8 * cw + i * RPP + lane / LPR) * (T * 128) + 8 * cl);
-            __syncwarp();
-            if (lane == 0) mbar_arrive(raw_empty(s));
+            for (int i = 0; i < RROWS / RPP; ++i)
+                w[i] = *reinterpret_cast<const uint2*>(rw + (r0 + i * RPP + lane / LPR) * (T * 128) + 8 * cl);
 #pragma unroll
-            for (int i = 0; i < 8 / RPP; ++i) {
+            for (int i = 0; i < RROWS / RPP; ++i) {
                 const int r = i * RPP + lane / LPR;
-                const float sr = __shfl_sync(FULL, sc, 8 * tile + r);
-                const uint2 a = codes_to_bf16(w[i].x, sr, p.e4m3), b = codes_to_bf16(w[i].y, sr, p.e4m3);
-                *reinterpret_cast<uint4*>(op + tile * RA_BYTES + box * 8192 + q8_sw128(8 * cw + r, unit)) =
-                    make_uint4(a.x, a.y, b.x, b.y);
+                const float sr = __shfl_sync(FULL, sc, RROWS * tile + r);
+                *reinterpret_cast<uint4*>(op + tile * RA_BYTES + box * 8192 + q8_sw128(r0 + r, unit)) =
+                    codes_to_bf16<E4M3>(w[i], sr);
             }
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int q = lane + 32 * i;
-                if (q >= 8 * units) break;
-                const int r = 8 * cw + q / units, j8 = q % units;
+            if (lane == 0) mbar_arrive(raw_empty(s));  // after the shuffles: every lane has read its codes
+            if (has_u) {
                 for (int piece = 0; piece < p.pieces; ++piece) {
                     uint32_t h[4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        h[j] = __byte_perm(__float_as_uint(u[i][2 * j]), __float_as_uint(u[i][2 * j + 1]), 0x7632);
-                        u[i][2 * j] = left_of(u[i][2 * j]);
-                        u[i][2 * j + 1] = left_of(u[i][2 * j + 1]);
+                        h[j] = __byte_perm(__float_as_uint(u[2 * j]), __float_as_uint(u[2 * j + 1]), 0x7632);
+                        u[2 * j] = left_of(u[2 * j]);
+                        u[2 * j + 1] = left_of(u[2 * j + 1]);
                     }
                     // the leading pieces fill the first box, the others the next two, end to end
-                    const int col8 = piece == 0 ? j8 : 8 + (piece - 1) * units + j8;
-                    *reinterpret_cast<uint4*>(op + T * RA_BYTES + (col8 >> 3) * RB_BOX + q8_sw128(r, col8 & 7)) =
+                    const int col8 = piece == 0 ? uj : 8 + (piece - 1) * units + uj;
+                    *reinterpret_cast<uint4*>(op + T * RA_BYTES + (col8 >> 3) * RB_BOX + q8_sw128(r0 + ur, col8 & 7)) =
                         make_uint4(h[0], h[1], h[2], h[3]);
                 }
             }
@@ -431,24 +472,20 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
     if (p.splits > 1) cluster_sync_all();  // peers keep their sums until every reader is done
 }
 
-template <int T>
-void launch(const RankCkpt8& a, RParams p, cudaStream_t s) {
-    typedef RShape<T> S;
-    static DeviceOnce once;
-    once([] { cudaFuncSetAttribute(rank_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM); });
-    const long tiles = (a.cols + T * 128 - 1) / (T * 128);
-    long splits = current_sm_count() / tiles;
-    if (splits > RMAX_SPLIT) splits = RMAX_SPLIT;
-    if (splits > p.nk) splits = p.nk;
-    if (splits < 1) splits = 1;
-    p.splits = (int)splits;
-    RMaps maps;
-    tc_make_map_raw(&maps.x, a.x.q, false, a.rows, a.cols, a.x.ldq, T * 128, RK);
+// How many clusters of `splits` CTAs run at once on the current device: the GPU's processing
+// clusters differ in size, so this is not the SM count over the size.  Asked once per device.
+template <int T, bool E4M3>
+int clusters_at_once(int splits) {
+    static std::atomic<int> known[64][RMAX_SPLIT + 1];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 1;
+    const bool cached = dev >= 0 && dev < 64;
+    int n = cached ? known[dev][splits].load(std::memory_order_relaxed) : 0;
+    if (n > 0) return n;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)tiles, (unsigned)splits, 1);
+    cfg.gridDim = dim3(1, (unsigned)splits, 1);
     cfg.blockDim = dim3(RTHREADS, 1, 1);
-    cfg.dynamicSmemBytes = S::SMEM;
-    cfg.stream = s;
+    cfg.dynamicSmemBytes = RShape<T>::SMEM;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 1;
@@ -456,7 +493,48 @@ void launch(const RankCkpt8& a, RParams p, cudaStream_t s) {
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, rank_kernel<T>, maps, p);
+    if (cudaOccupancyMaxActiveClusters(&n, rank_kernel<T, E4M3>, &cfg) != cudaSuccess || n < 1) {
+        cudaGetLastError();
+        return 1;
+    }
+    if (cached) known[dev][splits].store(n, std::memory_order_relaxed);
+    return n;
+}
+
+template <int T, bool E4M3>
+void launch(const RankCkpt8& a, RParams p, cudaStream_t s) {
+    typedef RShape<T> S;
+    static DeviceOnce once;
+    once([] {
+        cudaFuncSetAttribute(rank_kernel<T, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+    });
+    const long tiles = (a.cols + T * 128 - 1) / (T * 128);
+    // slices per tile: the least rounds of clusters times blocks of a slice
+    p.splits = 1;
+    long best = -1;
+    for (int n = 1; n <= RMAX_SPLIT && n <= p.nk; ++n) {
+        const long at_once = clusters_at_once<T, E4M3>(n);
+        const long cost = (tiles + at_once - 1) / at_once * ((p.nk + n - 1) / n);
+        if (best < 0 || cost < best) {
+            best = cost;
+            p.splits = n;
+        }
+    }
+    RMaps maps;
+    tc_make_map_raw(&maps.x, a.x.q, false, a.rows, a.cols, a.x.ldq, T * 128, RK);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)tiles, (unsigned)p.splits, 1);
+    cfg.blockDim = dim3(RTHREADS, 1, 1);
+    cfg.dynamicSmemBytes = S::SMEM;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1;
+    attr[0].val.clusterDim.y = (unsigned)p.splits;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, rank_kernel<T, E4M3>, maps, p);
 }
 
 }  // namespace
@@ -471,13 +549,13 @@ void rank_ckpt8(const RankCkpt8& a, cudaStream_t s) {
     p.cols = a.cols;
     p.u = a.u.p; p.u_type = a.u.type; p.u_vec = vec4(a.u) ? 1 : 0; p.ldu = a.u.ld;
     p.pieces = a.u.type == OP_F32 ? 3 : a.u.type == OP_F16 ? 2 : 1;
-    p.scale = a.x.scale; p.lds = a.x.lds; p.e4m3 = a.x.e4m3 ? 1 : 0; p.alpha = a.alpha;
+    p.scale = a.x.scale; p.lds = a.x.lds; p.alpha = a.alpha;
     p.c = a.c; p.ldc = a.ldc; p.c_vec = vec4(a.c) && a.ldc % 4 == 0 ? 1 : 0; p.accumulate = a.accumulate ? 1 : 0;
     p.splits = 1; p.status = a.status;
     // 256 columns a CTA halve the work on U per code, where that still leaves CTAs for most SMs
     const long wide = (a.cols + 255) / 256;
-    if (wide * RMAX_SPLIT >= current_sm_count()) launch<2>(a, p, s);
-    else launch<1>(a, p, s);
+    if (wide * RMAX_SPLIT >= current_sm_count()) a.x.e4m3 ? launch<2, true>(a, p, s) : launch<2, false>(a, p, s);
+    else a.x.e4m3 ? launch<1, true>(a, p, s) : launch<1, false>(a, p, s);
 }
 
 }  // namespace act
