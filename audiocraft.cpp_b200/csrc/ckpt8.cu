@@ -7,6 +7,8 @@
 // 128 columns and RPW neighbouring rows of it at a time: the block's maximum is one warp
 // reduction, the loads of all rows are in flight together, and the rows' scales, which lie next
 // to each other (block-major), leave as one store.
+#include <type_traits>
+
 #include "ckpt8.cuh"
 
 namespace act {
@@ -21,11 +23,12 @@ constexpr int THREADS = 256;
 // A warp's block column and its first row group; warps beyond the last whole set of block
 // columns have none
 struct Place {
-    int chunk, n;    // block column, columns of the row from its first one
-    long row, step;  // first row, rows between two groups of this warp
+    int chunk, n;         // block column; columns of the row from the lane's first one
+    long col, row, step;  // the lane's first column, first row, rows between two groups of this warp
     bool any;
 };
-__device__ __forceinline__ Place place(long rows, long cols) {
+template <bool VEC>
+__device__ __forceinline__ Place place(long cols) {
     const unsigned warp = blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5), nwarps = gridDim.x * (THREADS / 32);
     const unsigned chunks = (unsigned)((cols + BLOCK - 1) / BLOCK), lanes = nwarps / chunks;
     Place p;
@@ -33,36 +36,63 @@ __device__ __forceinline__ Place place(long rows, long cols) {
     p.row = (long)(warp / chunks) * RPW;
     p.step = (long)lanes * RPW;
     p.any = warp / chunks < lanes;
-    const long left = cols - (long)p.chunk * BLOCK;
-    p.n = left < BLOCK ? (int)left : BLOCK;
+    p.col = (long)p.chunk * BLOCK + first_col<VEC>(threadIdx.x & 31);
+    p.n = cols - p.col < BLOCK ? (int)(cols - p.col) : BLOCK;
     return p;
 }
 
+// body(place, row, rows, whole) for each of the warp's groups of up to RPW rows
+template <bool VEC, typename Body>
+__device__ __forceinline__ void each_group(long rows, long cols, Body&& body) {
+    const Place p = place<VEC>(cols);
+    if (!p.any) return;
+    long row = p.row;
+    for (; row + RPW <= rows; row += p.step) body(p, row, RPW, std::true_type());
+    if (row < rows) body(p, row, (int)(rows - row), std::false_type());
+}
+
 // the scales of up to RPW rows: lane r holds row r's
-__device__ __forceinline__ void store_scales(const Q8& t, int chunk, long row, int nr, int lane, const uint32_t* s) {
+__device__ __forceinline__ void store_scales(const Q8& t, int chunk, long row, int nr, const uint32_t* s) {
+    const int lane = threadIdx.x & 31;
     uint32_t mine = s[0];
 #pragma unroll
     for (int r = 1; r < RPW; ++r) mine = lane == r ? s[r] : mine;
     if (lane < nr) t.scale[(long)chunk * t.lds + row + lane] = __uint_as_float(mine);
 }
 
+// v: RPW rows of a block, -> codes and scales
+template <bool VEC, bool FULL>
+__device__ __forceinline__ void store_rows(const Q8& t, const Place& p, long row, int nr, const float (*v)[4],
+                                           bool e4m3) {
+    uint32_t s[RPW], top[RPW], most = 0;
+    uint8_t* q = t.q + row * t.ldq + p.col;
+#pragma unroll
+    for (int r = 0; r < RPW; ++r) {
+        top[r] = __reduce_max_sync(FULL_WARP, largest(v[r]));
+        most = max(most, top[r]);
+    }
+    const bool bad = most >= 0x7f800000u;  // one test for all rows: something is not finite
+    if (bad)
+#pragma unroll
+        for (int r = 0; r < RPW; ++r) top[r] = __reduce_max_sync(FULL_WARP, largest_finite(v[r]));
+#pragma unroll
+    for (int r = 0; r < RPW; ++r) {
+        s[r] = scale_bits(top[r], e4m3);
+        store_codes<VEC>(q + r * t.ldq, FULL || r < nr ? p.n : 0, encode4(v[r], inverse_pow2(s[r]), e4m3, bad));
+    }
+    store_scales(t, p.chunk, row, nr, s);
+}
+
 template <typename T, bool VEC, bool E4M3>
 __global__ void __launch_bounds__(THREADS) store_kernel(const T* x, long ldx, long rows, long cols, Q8 out) {
-    const int lane = threadIdx.x & 31;
-    const Place p = place(rows, cols);
-    if (!p.any) return;
-    const long c0 = (long)p.chunk * BLOCK;
-    for (long row = p.row; row < rows; row += p.step) {
-        const int nr = rows - row < RPW ? (int)(rows - row) : RPW;
+    each_group<VEC>(rows, cols, [&](const Place& p, long row, int nr, auto full) {
+        constexpr bool FULL = decltype(full)::value;
         float v[RPW][4];
-        uint32_t s[RPW];
+        const T* at = x + row * ldx + p.col;
 #pragma unroll
-        for (int r = 0; r < RPW; ++r) load4<T, VEC>(x + (row + r) * ldx + c0, r < nr ? p.n : 0, lane, v[r]);
-#pragma unroll
-        for (int r = 0; r < RPW; ++r)
-            s[r] = store_block<VEC>(out.q + (row + r) * out.ldq + c0, r < nr ? p.n : 0, lane, v[r], E4M3);
-        store_scales(out, p.chunk, row, nr, lane, s);
-    }
+        for (int r = 0; r < RPW; ++r) load4<T, VEC>(at + r * ldx, FULL || r < nr ? p.n : 0, v[r]);
+        store_rows<VEC, FULL>(out, p, row, nr, v, E4M3);
+    });
 }
 
 // one CTA per 128 x 128 block: a first pass for the maximum, a second that finds the block in L1
@@ -70,19 +100,19 @@ template <typename T, bool VEC, bool E4M3>
 __global__ void __launch_bounds__(THREADS) store_square_kernel(const T* x, long ldx, long rows, long cols, Q8 out) {
     __shared__ uint32_t top[THREADS / 32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const long c0 = (long)blockIdx.x * BLOCK;
+    const long c0 = (long)blockIdx.x * BLOCK + first_col<VEC>(lane);
     const int n = cols - c0 < BLOCK ? (int)(cols - c0) : BLOCK;
     for (long rb = blockIdx.y; rb * BLOCK < rows; rb += gridDim.y) {
         const long r0 = rb * BLOCK, r1 = r0 + BLOCK < rows ? r0 + BLOCK : rows;
         uint32_t m = 0, any = 0;
         for (long r = r0 + warp; r < r1; r += THREADS / 32) {
             float v[4];
-            load4<T, VEC>(x + r * ldx + c0, n, lane, v);
+            load4<T, VEC>(x + r * ldx + c0, n, v);
             m = max(m, largest_finite(v));
             any = max(any, largest(v));
         }
         const bool bad = __syncthreads_or(any >= 0x7f800000u);
-        m = __reduce_max_sync(FULL, m);
+        m = __reduce_max_sync(FULL_WARP, m);
         if (lane == 0) top[warp] = m;
         __syncthreads();
 #pragma unroll
@@ -90,8 +120,8 @@ __global__ void __launch_bounds__(THREADS) store_square_kernel(const T* x, long 
         const uint32_t s = scale_bits(m, E4M3);
         for (long r = r0 + warp; r < r1; r += THREADS / 32) {
             float v[4];
-            load4<T, VEC>(x + r * ldx + c0, n, lane, v);
-            store_codes<VEC>(out.q + r * out.ldq + c0, n, lane, encode4(v, inverse_pow2(s), E4M3, bad));
+            load4<T, VEC>(x + r * ldx + c0, n, v);
+            store_codes<VEC>(out.q + r * out.ldq + c0, n, encode4(v, inverse_pow2(s), E4M3, bad));
         }
         if (threadIdx.x == 0) out.scale[(long)blockIdx.x * out.lds + rb] = __uint_as_float(s);
     }
@@ -100,94 +130,82 @@ __global__ void __launch_bounds__(THREADS) store_square_kernel(const T* x, long 
 // shift: log2 of the block's rows
 template <typename T, bool VEC, bool E4M3>
 __global__ void __launch_bounds__(THREADS) load_kernel(Q8 in, long rows, long cols, int shift, T* y, long ldy) {
-    const int lane = threadIdx.x & 31;
-    const Place p = place(rows, cols);
-    if (!p.any) return;
-    const long c0 = (long)p.chunk * BLOCK;
-    for (long row = p.row; row < rows; row += p.step) {
-        const int nr = rows - row < RPW ? (int)(rows - row) : RPW;
-        float v[RPW][4], s[RPW];
+    each_group<VEC>(rows, cols, [&](const Place& p, long row, int nr, auto full) {
+        constexpr bool FULL = decltype(full)::value;
         uint32_t w[RPW];
+        float s[RPW];
+        const uint8_t* q = in.q + row * in.ldq + p.col;
+        const float* scale = in.scale + (long)p.chunk * in.lds;
+        T* at = y + row * ldy + p.col;
 #pragma unroll
         for (int r = 0; r < RPW; ++r) {
-            w[r] = load_codes<VEC>(in.q + (row + r) * in.ldq + c0, r < nr ? p.n : 0, lane);
-            s[r] = r < nr ? in.scale[(long)p.chunk * in.lds + ((row + r) >> shift)] : 0.f;
+            w[r] = load_codes<VEC>(q + r * in.ldq, FULL || r < nr ? p.n : 0);
+            s[r] = FULL || r < nr ? scale[(row + r) >> shift] : 0.f;
         }
 #pragma unroll
         for (int r = 0; r < RPW; ++r) {
-            decode4(w[r], E4M3, v[r]);
+            float v[4];
+            decode4(w[r], E4M3, v);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[r][i] *= s[r];
-            store4<T, VEC>(y + (row + r) * ldy + c0, r < nr ? p.n : 0, lane, v[r]);
+            for (int i = 0; i < 4; ++i) v[i] *= s[r];
+            store4<T, VEC>(at + r * ldy, FULL || r < nr ? p.n : 0, v);
         }
-    }
+    });
 }
 
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(THREADS)
     gelu_fwd_kernel(const T* z, long ldz, long rows, long cols, T* g, long ldg, Q8 g8, Q8 z8) {
-    const int lane = threadIdx.x & 31;
-    const Place p = place(rows, cols);
-    if (!p.any) return;
-    const long c0 = (long)p.chunk * BLOCK;
-    for (long row = p.row; row < rows; row += p.step) {
-        const int nr = rows - row < RPW ? (int)(rows - row) : RPW;
+    each_group<VEC>(rows, cols, [&](const Place& p, long row, int nr, auto full) {
+        constexpr bool FULL = decltype(full)::value;
         float v[RPW][4];
-        uint32_t s[RPW];
+        const T* at = z + row * ldz + p.col;
 #pragma unroll
-        for (int r = 0; r < RPW; ++r) load4<T, VEC>(z + (row + r) * ldz + c0, r < nr ? p.n : 0, lane, v[r]);
+        for (int r = 0; r < RPW; ++r) load4<T, VEC>(at + r * ldz, FULL || r < nr ? p.n : 0, v[r]);
+        store_rows<VEC, FULL>(z8, p, row, nr, v, z8.e4m3);
 #pragma unroll
         for (int r = 0; r < RPW; ++r)
-            s[r] = store_block<VEC>(z8.q + (row + r) * z8.ldq + c0, r < nr ? p.n : 0, lane, v[r], z8.e4m3);
-        store_scales(z8, p.chunk, row, nr, lane, s);
-#pragma unroll
-        for (int r = 0; r < RPW; ++r) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[r][i] = gelu(v[r][i]);
-            if (g) store4<T, VEC>(g + (row + r) * ldg + c0, r < nr ? p.n : 0, lane, v[r]);
-        }
-        if (g8.q) {
+        if (g) {
+            T* to = g + row * ldg + p.col;
 #pragma unroll
-            for (int r = 0; r < RPW; ++r)
-                s[r] = store_block<VEC>(g8.q + (row + r) * g8.ldq + c0, r < nr ? p.n : 0, lane, v[r], g8.e4m3);
-            store_scales(g8, p.chunk, row, nr, lane, s);
+            for (int r = 0; r < RPW; ++r) store4<T, VEC>(to + r * ldg, FULL || r < nr ? p.n : 0, v[r]);
         }
-    }
+        if (g8.q) store_rows<VEC, FULL>(g8, p, row, nr, v, g8.e4m3);
+    });
 }
 
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(THREADS)
     gelu_bwd_kernel(const T* dg, long lddg, Q8 z8, long rows, long cols, T* dz, long lddz, Q8 dz8) {
-    const int lane = threadIdx.x & 31;
-    const Place p = place(rows, cols);
-    if (!p.any) return;
-    const long c0 = (long)p.chunk * BLOCK;
-    for (long row = p.row; row < rows; row += p.step) {
-        const int nr = rows - row < RPW ? (int)(rows - row) : RPW;
+    each_group<VEC>(rows, cols, [&](const Place& p, long row, int nr, auto full) {
+        constexpr bool FULL = decltype(full)::value;
         float v[RPW][4], s[RPW];
         uint32_t w[RPW];
+        const T* at = dg + row * lddg + p.col;
+        const uint8_t* q = z8.q + row * z8.ldq + p.col;
+        const float* scale = z8.scale + (long)p.chunk * z8.lds + row;
 #pragma unroll
         for (int r = 0; r < RPW; ++r) {
-            load4<T, VEC>(dg + (row + r) * lddg + c0, r < nr ? p.n : 0, lane, v[r]);
-            w[r] = load_codes<VEC>(z8.q + (row + r) * z8.ldq + c0, r < nr ? p.n : 0, lane);
-            s[r] = r < nr ? z8.scale[(long)p.chunk * z8.lds + row + r] : 0.f;
+            load4<T, VEC>(at + r * lddg, FULL || r < nr ? p.n : 0, v[r]);
+            w[r] = load_codes<VEC>(q + r * z8.ldq, FULL || r < nr ? p.n : 0);
+            s[r] = FULL || r < nr ? scale[r] : 0.f;
         }
 #pragma unroll
         for (int r = 0; r < RPW; ++r) {
-            float z[4];
-            decode4(w[r], z8.e4m3, z);
+            float k[4];
+            decode4(w[r], z8.e4m3, k);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[r][i] *= gelu_grad(z[i] * s[r]);
-            if (dz) store4<T, VEC>(dz + (row + r) * lddz + c0, r < nr ? p.n : 0, lane, v[r]);
+            for (int i = 0; i < 4; ++i) v[r][i] *= gelu_grad(k[i] * s[r]);
         }
-        if (dz8.q) {
-            uint32_t sb[RPW];
+        if (dz) {
+            T* to = dz + row * lddz + p.col;
 #pragma unroll
-            for (int r = 0; r < RPW; ++r)
-                sb[r] = store_block<VEC>(dz8.q + (row + r) * dz8.ldq + c0, r < nr ? p.n : 0, lane, v[r], dz8.e4m3);
-            store_scales(dz8, p.chunk, row, nr, lane, sb);
+            for (int r = 0; r < RPW; ++r) store4<T, VEC>(to + r * lddz, FULL || r < nr ? p.n : 0, v[r]);
         }
-    }
+        if (dz8.q) store_rows<VEC, FULL>(dz8, p, row, nr, v, dz8.e4m3);
+    });
 }
 
 // enough warps to fill the GPU (eight CTAs of 256 an SM) or, if there is less, one row group each;
@@ -216,7 +234,7 @@ void by_type(int type, Fn&& f) {
 }  // namespace
 
 void ckpt8_store(const OpTensor& x, long rows, long cols, int block_rows, const Q8& out, cudaStream_t s) {
-    const bool v = vec4(x) && vec4(out);
+    const bool v = cols % 4 == 0 && vec4(x) && vec4(out);
     by_type(x.type, [&](auto t) {
         typedef decltype(t) T;
         if (block_rows == 1) {
@@ -234,7 +252,7 @@ void ckpt8_store(const OpTensor& x, long rows, long cols, int block_rows, const 
 }
 
 void ckpt8_load(const Q8& in, long rows, long cols, int block_rows, const OpTensor& y, cudaStream_t s) {
-    const bool v = vec4(y) && vec4(in);
+    const bool v = cols % 4 == 0 && vec4(y) && vec4(in);
     by_type(y.type, [&](auto t) {
         typedef decltype(t) T;
         auto* k = v ? (in.e4m3 ? load_kernel<T, true, true> : load_kernel<T, true, false>)
@@ -245,7 +263,7 @@ void ckpt8_load(const Q8& in, long rows, long cols, int block_rows, const OpTens
 
 void gelu_ckpt8_fwd(const OpTensor& z, long rows, long cols, const OpTensor& g, const Q8& g8, const Q8& z8,
                     cudaStream_t s) {
-    const bool v = vec4(z) && vec4(g) && vec4(g8) && vec4(z8);
+    const bool v = cols % 4 == 0 && vec4(z) && vec4(g) && vec4(g8) && vec4(z8);
     by_type(z.type, [&](auto t) {
         typedef decltype(t) T;
         auto* k = v ? gelu_fwd_kernel<T, true> : gelu_fwd_kernel<T, false>;
@@ -255,7 +273,7 @@ void gelu_ckpt8_fwd(const OpTensor& z, long rows, long cols, const OpTensor& g, 
 
 void gelu_ckpt8_bwd(const OpTensor& dg, const Q8& z8, long rows, long cols, const OpTensor& dz, const Q8& dz8,
                     cudaStream_t s) {
-    const bool v = vec4(dg) && vec4(dz) && vec4(z8) && vec4(dz8);
+    const bool v = cols % 4 == 0 && vec4(dg) && vec4(dz) && vec4(z8) && vec4(dz8);
     by_type(dg.type, [&](auto t) {
         typedef decltype(t) T;
         auto* k = v ? gelu_bwd_kernel<T, true> : gelu_bwd_kernel<T, false>;

@@ -11,16 +11,21 @@ namespace act {
 namespace c8 {
 
 constexpr int BLOCK = 128;  // columns of a block
-constexpr uint32_t FULL = 0xffffffffu;
+constexpr uint32_t FULL_WARP = 0xffffffffu;
 
 // ---------------------------------------------------------------------------------------
-// Four elements of a row per lane, one block of 128 columns per warp.  With VEC the lane owns the
-// columns 4 lane .. 4 lane + 3 and moves them as one word when all four exist (bases and strides
-// are multiples of four elements); without, it owns lane, lane + 32, .. so that a warp's scalar
-// accesses still cover whole sectors.
+// Four elements of a row per lane, one block of 128 columns per warp.  With VEC (bases, strides and
+// columns are multiples of four elements) the lane owns the columns 4 lane .. 4 lane + 3, which
+// exist all or not at all, and moves them as one word; without, it owns lane, lane + 32, .. so
+// that a warp's scalar accesses still cover whole sectors.  Pointers are the lane's own (block's
+// first element plus first_col) and `n` counts the columns of the row from the lane's first one.
 template <bool VEC>
-__device__ __forceinline__ int lane_col(int lane, int i) {
-    return VEC ? 4 * lane + i : lane + 32 * i;
+__device__ __forceinline__ int first_col(int lane) {
+    return VEC ? 4 * lane : lane;
+}
+template <bool VEC>
+__device__ __forceinline__ constexpr int elem(int i) {
+    return VEC ? i : 32 * i;
 }
 
 __device__ __forceinline__ float to_f32(float v) { return v; }
@@ -35,64 +40,137 @@ __device__ __forceinline__ f16 from_f32<f16>(float v) { return __float2half_rn(v
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-template <int BYTES>
-struct Word4;
-template <>
-struct Word4<4> { typedef uint4 type; };
-template <>
-struct Word4<2> { typedef uint2 type; };
-template <>
-struct Word4<1> { typedef uint32_t type; };
+// four neighbouring elements as one word
+__device__ __forceinline__ void unpack4(const float4& w, float v[4], float) {
+    v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w;
+}
+__device__ __forceinline__ void unpack4(const uint2& w, float v[4], f16) {
+    const float2 a = unpack_f16(w.x), b = unpack_f16(w.y);
+    v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+}
+__device__ __forceinline__ void unpack4(const uint2& w, float v[4], __nv_bfloat16) {
+    v[0] = __uint_as_float(w.x << 16); v[1] = __uint_as_float(w.x & 0xffff0000u);
+    v[2] = __uint_as_float(w.y << 16); v[3] = __uint_as_float(w.y & 0xffff0000u);
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ float4 pack4(const float v[4], float) { return make_float4(v[0], v[1], v[2], v[3]); }
+__device__ __forceinline__ uint2 pack4(const float v[4], f16) {
+    return make_uint2(pack_f16(v[0], v[1]), pack_f16(v[2], v[3]));
+}
+__device__ __forceinline__ uint2 pack4(const float v[4], __nv_bfloat16) {
+    return make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+}
 
-// p: the block's first element; n: columns of the row from there (may exceed 128); missing
-// columns read as 0
+// what a lane holds of a block as it lies in memory, for loads issued well before their use;
+// missing columns read as 0
 template <typename T, bool VEC>
-__device__ __forceinline__ void load4(const T* p, int n, int lane, float v[4]) {
-    if (VEC && 4 * lane + 3 < n) {
-        typedef typename Word4<sizeof(T)>::type W;
-        const W w = *reinterpret_cast<const W*>(p + 4 * lane);
-        const T* e = reinterpret_cast<const T*>(&w);
+struct Raw4 {
+    typedef decltype(pack4((const float*)nullptr, T())) Word;
+    Word w;
+    __device__ __forceinline__ void load(const T* p, int n) {
+        w = Word();
+        if (n > 0) w = *reinterpret_cast<const Word*>(p);
+    }
+    __device__ __forceinline__ void values(float v[4]) const { unpack4(w, v, T()); }
+};
+template <typename T>
+struct Raw4<T, false> {
+    T e[4];
+    __device__ __forceinline__ void load(const T* p, int n) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[i] = 32 * i < n ? p[32 * i] : T(0.f);
+    }
+    __device__ __forceinline__ void values(float v[4]) const {
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = to_f32(e[i]);
-        return;
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int c = lane_col<VEC>(lane, i);
-        v[i] = c < n ? to_f32(p[c]) : 0.f;
-    }
-}
-
+};
 template <typename T, bool VEC>
-__device__ __forceinline__ void store4(T* p, int n, int lane, const float v[4]) {
-    if (VEC && 4 * lane + 3 < n) {
-        typedef typename Word4<sizeof(T)>::type W;
-        W w;
-        T* e = reinterpret_cast<T*>(&w);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) e[i] = from_f32<T>(v[i]);
-        *reinterpret_cast<W*>(p + 4 * lane) = w;
+__device__ __forceinline__ void load4(const T* p, int n, float v[4]) {
+    Raw4<T, VEC> r;
+    r.load(p, n);
+    r.values(v);
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void store4(T* p, int n, const float v[4]) {
+    typedef decltype(pack4(v, T())) Word;
+    if (VEC) {
+        if (n > 0) *reinterpret_cast<Word*>(p) = pack4(v, T());
         return;
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int c = lane_col<VEC>(lane, i);
-        if (c < n) p[c] = from_f32<T>(v[i]);
+    for (int i = 0; i < 4; ++i)
+        if (32 * i < n) p[32 * i] = from_f32<T>(v[i]);
+}
+// parameters that no kernel here writes: loads that may move across its stores
+template <bool VEC>
+__device__ __forceinline__ void load4_const(const float* p, int n, float v[4]) {
+    if (VEC) {
+        float4 w = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (n > 0) w = __ldg(reinterpret_cast<const float4*>(p));
+        unpack4(w, v, float());
+        return;
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = 32 * i < n ? __ldg(p + 32 * i) : 0.f;
+}
+// elements of B bytes: fp32, or f16 / bf16 told apart at run time
+template <int B, bool VEC>
+__device__ __forceinline__ void store4_bytes(char* p, bool half, int n, const float v[4]) {
+    if (B == 4) return store4<float, VEC>(reinterpret_cast<float*>(p), n, v);
+    if (VEC) {
+        const uint2 a = pack4(v, f16()), b = pack4(v, __nv_bfloat16());
+        if (n > 0) *reinterpret_cast<uint2*>(p) = half ? a : b;
+        return;
+    }
+    if (half) store4<f16, VEC>(reinterpret_cast<f16*>(p), n, v);
+    else store4<__nv_bfloat16, VEC>(reinterpret_cast<__nv_bfloat16*>(p), n, v);
+}
+template <int B, bool VEC>
+__device__ __forceinline__ void load4_bytes(const char* p, bool half, int n, float v[4]) {
+    if (B == 4) return load4<float, VEC>(reinterpret_cast<const float*>(p), n, v);
+    if (half) load4<f16, VEC>(reinterpret_cast<const f16*>(p), n, v);
+    else load4<__nv_bfloat16, VEC>(reinterpret_cast<const __nv_bfloat16*>(p), n, v);
 }
 
-// the same with the element type known at run time only (one uniform branch per four elements)
-template <bool VEC>
-__device__ __forceinline__ void store4_as(void* base, int type, long off, int n, int lane, const float v[4]) {
-    if (type == OP_F16) store4<f16, VEC>(static_cast<f16*>(base) + off, n, lane, v);
-    else if (type == OP_BF16) store4<__nv_bfloat16, VEC>(static_cast<__nv_bfloat16*>(base) + off, n, lane, v);
-    else store4<float, VEC>(static_cast<float*>(base) + off, n, lane, v);
+// ---------------------------------------------------------------------------------------
+// Two fp32 in a 64-bit register: one instruction works on both.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(__float_as_uint(lo)), "r"(__float_as_uint(hi)));
+    return r;
 }
-template <bool VEC>
-__device__ __forceinline__ void load4_as(const void* base, int type, long off, int n, int lane, float v[4]) {
-    if (type == OP_F16) load4<f16, VEC>(static_cast<const f16*>(base) + off, n, lane, v);
-    else if (type == OP_BF16) load4<__nv_bfloat16, VEC>(static_cast<const __nv_bfloat16*>(base) + off, n, lane, v);
-    else load4<float, VEC>(static_cast<const float*>(base) + off, n, lane, v);
+__device__ __forceinline__ uint64_t pair(float v) { return pair(v, v); }
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+    uint32_t a, b;
+    asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(v));
+    return make_float2(__uint_as_float(a), __uint_as_float(b));
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ void pairs(const float v[4], uint64_t o[2]) {
+    o[0] = pair(v[0], v[1]);
+    o[1] = pair(v[2], v[3]);
+}
+__device__ __forceinline__ void unpairs(const uint64_t v[2], float o[4]) {
+    const float2 a = unpair(v[0]), b = unpair(v[1]);
+    o[0] = a.x; o[1] = a.y; o[2] = b.x; o[3] = b.y;
 }
 
 // ---------------------------------------------------------------------------------------
@@ -117,8 +195,13 @@ struct Top {
     uint32_t bits;
     bool bad;
 };
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
 __device__ __forceinline__ uint32_t largest(const float v[4]) {
-    return max(max(abs_bits(v[0]), abs_bits(v[1])), max(abs_bits(v[2]), abs_bits(v[3])));
+    return abs_bits(max_nan(max_nan(fabsf(v[0]), fabsf(v[1])), max_nan(fabsf(v[2]), fabsf(v[3]))));
 }
 __device__ __forceinline__ uint32_t largest_finite(const float v[4]) {
     uint32_t m = 0;
@@ -128,9 +211,9 @@ __device__ __forceinline__ uint32_t largest_finite(const float v[4]) {
 }
 __device__ __forceinline__ Top warp_top(const float v[4]) {
     Top t;
-    t.bits = __reduce_max_sync(FULL, largest(v));
+    t.bits = __reduce_max_sync(FULL_WARP, largest(v));
     t.bad = t.bits >= 0x7f800000u;
-    if (t.bad) t.bits = __reduce_max_sync(FULL, largest_finite(v));
+    if (t.bad) t.bits = __reduce_max_sync(FULL_WARP, largest_finite(v));
     return t;
 }
 
@@ -159,7 +242,8 @@ __device__ __forceinline__ uint32_t encode4(const float v[4], float inv, bool e4
     return __byte_perm(__byte_perm(r[0], r[1], 0x0040), __byte_perm(r[2], r[3], 0x0040), 0x5410);
 }
 
-// four codes -> the whole numbers / floats they stand for before scaling (I8 -128: NaN)
+// Four codes -> the whole numbers / floats they stand for before scaling (I8 -128: NaN).  I8: the
+// code plus 128 goes into the low byte of the float 2^23, from which 2^23 + 128 is taken (exact).
 __device__ __forceinline__ void decode4(uint32_t w, bool e4m3, float v[4]) {
     if (e4m3) {
         const __half2 a = __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3));
@@ -168,52 +252,46 @@ __device__ __forceinline__ void decode4(uint32_t w, bool e4m3, float v[4]) {
         v[0] = fa.x; v[1] = fa.y; v[2] = fb.x; v[3] = fb.y;
         return;
     }
+    const uint32_t x = w ^ 0x80808080u;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int q = (int)(int8_t)(w >> (8 * i));
-        v[i] = q == -128 ? __int_as_float(0x7fc00000) : (float)q;
-    }
+    for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(__byte_perm(x, 0x4b000000u, 0x7650 + i)) - 8388736.0f;
+    if ((x - 0x01010101u) & ~x & 0x80808080u)  // a zero byte of x (a borrow may flag the one above too)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (((x >> (8 * i)) & 0xffu) == 0) v[i] = __int_as_float(0x7fc00000);
 }
 
-// codes of one block of a row
+// a lane's codes of one block of a row
 template <bool VEC>
-__device__ __forceinline__ void store_codes(uint8_t* p, int n, int lane, uint32_t w) {
-    if (VEC && 4 * lane + 3 < n) {
-        *reinterpret_cast<uint32_t*>(p + 4 * lane) = w;
+__device__ __forceinline__ void store_codes(uint8_t* p, int n, uint32_t w) {
+    if (VEC) {
+        if (n > 0) *reinterpret_cast<uint32_t*>(p) = w;
         return;
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int c = lane_col<VEC>(lane, i);
-        if (c < n) p[c] = (uint8_t)(w >> (8 * i));
-    }
+    for (int i = 0; i < 4; ++i)
+        if (32 * i < n) p[32 * i] = (uint8_t)(w >> (8 * i));
 }
 template <bool VEC>
-__device__ __forceinline__ uint32_t load_codes(const uint8_t* p, int n, int lane) {
-    if (VEC && 4 * lane + 3 < n) return *reinterpret_cast<const uint32_t*>(p + 4 * lane);
+__device__ __forceinline__ uint32_t load_codes(const uint8_t* p, int n) {
     uint32_t w = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int c = lane_col<VEC>(lane, i);
-        if (c < n) w |= (uint32_t)p[c] << (8 * i);
+    if (VEC) {
+        if (n > 0) w = *reinterpret_cast<const uint32_t*>(p);
+        return w;
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (32 * i < n) w |= (uint32_t)p[32 * i] << (8 * i);
     return w;
 }
 
 // quantise and store one block held by a warp; returns the scale's bits (the caller stores it)
 template <bool VEC>
-__device__ __forceinline__ uint32_t store_block(uint8_t* p, int n, int lane, const float v[4], bool e4m3) {
+__device__ __forceinline__ uint32_t store_block(uint8_t* p, int n, const float v[4], bool e4m3) {
     const Top t = warp_top(v);
     const uint32_t s = scale_bits(t.bits, e4m3);
-    store_codes<VEC>(p, n, lane, encode4(v, inverse_pow2(s), e4m3, t.bad));
+    store_codes<VEC>(p, n, encode4(v, inverse_pow2(s), e4m3, t.bad));
     return s;
-}
-
-template <bool VEC>
-__device__ __forceinline__ void load_block(const uint8_t* p, int n, int lane, float scale, bool e4m3, float v[4]) {
-    decode4(load_codes<VEC>(p, n, lane), e4m3, v);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] *= scale;
 }
 
 // ---------------------------------------------------------------------------------------

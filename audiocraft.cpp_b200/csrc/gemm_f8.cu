@@ -89,13 +89,16 @@ __device__ __forceinline__ void put4(const Params& p, long m, long n, float4 f) 
         for (int i = 0; i < 4; ++i)
             if (i < left) v[i] += p.bias[n + i];
     if (p.vec && left == 4) {
+        char* y = static_cast<char*>(p.y) + at * (p.y_type == OP_F32 ? 4 : 2);
         if (p.accumulate) {
             float o[4];
-            load4_as<true>(p.y, p.y_type, at, 4, 0, o);
+            if (p.y_type == OP_F32) load4_bytes<4, true>(y, false, 4, o);
+            else load4_bytes<2, true>(y, p.y_type == OP_F16, 4, o);
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[i] += o[i];
         }
-        store4_as<true>(p.y, p.y_type, at, 4, 0, v);
+        if (p.y_type == OP_F32) store4_bytes<4, true>(y, false, 4, v);
+        else store4_bytes<2, true>(y, p.y_type == OP_F16, 4, v);
         return;
     }
     for (int i = 0; i < left; ++i) put_value(p, at + i, p.accumulate ? old_value(p, at + i) + v[i] : v[i]);
@@ -230,14 +233,14 @@ __global__ void __launch_bounds__(NTHREADS, 1) gemm_f8_kernel(const __grid_const
             for (int i = 0; i < S::HALF / 2; ++i) acc[i] = 0;
             float a = sx[0], w = sw[0];
             for (int kb = 0; kb < p.nk; ++kb) {
-                const uint64_t sc = pack2(a * w);
+                const uint64_t sc = pair(a * w);
                 if (kb + 1 < p.nk) {
                     a = sx[(long)(kb + 1) * p.ldsx];
                     w = sw[(long)(kb + 1) * wstep];
                 }
                 bool got = true;
                 if (lane == 0) got = mbar_wait_inline(tfull(b), bph, p.status, 34);
-                if (!__shfl_sync(FULL, got ? 1 : 0, 0)) { ok = false; break; }
+                if (!__shfl_sync(FULL_WARP, got ? 1 : 0, 0)) { ok = false; break; }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 uint32_t r[2][16];
                 tmem_ld16_start(tcol + b * BN, r[0]);
@@ -251,7 +254,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) gemm_f8_kernel(const __grid_const
                         if (lane == 0) mbar_arrive(tempty(b));
                     }
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) fma2(acc[8 * c + i], r[c & 1][2 * i], r[c & 1][2 * i + 1], sc);
+                    for (int i = 0; i < 8; ++i)
+                        acc[8 * c + i] = fma2(pair(__uint_as_float(r[c & 1][2 * i]), __uint_as_float(r[c & 1][2 * i + 1])), sc, acc[8 * c + i]);
                 }
                 b ^= 1;
                 if (b == 0) bph ^= 1;
@@ -264,7 +268,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) gemm_f8_kernel(const __grid_const
                 __syncwarp();
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const float2 u = unpack2(acc[16 * c + 2 * i]), v = unpack2(acc[16 * c + 2 * i + 1]);
+                    const float2 u = unpair(acc[16 * c + 2 * i]), v = unpair(acc[16 * c + 2 * i + 1]);
                     *reinterpret_cast<float4*>(stage + lane * EPI_LD + 4 * i) = make_float4(u.x, u.y, v.x, v.y);
                 }
                 __syncwarp();

@@ -76,37 +76,18 @@ struct RMaps {
     CUtensorMap x;
 };
 
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
 __device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
-__device__ __forceinline__ uint64_t pair(float lo, float hi) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(__float_as_uint(lo)), "r"(__float_as_uint(hi)));
-    return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint32_t pack_bf16(uint64_t v) {
-    const float2 f = unpack2(v);
+__device__ __forceinline__ uint32_t pair_bf16(uint64_t v) {
+    const float2 f = unpair(v);
     return pack_bf16(f.x, f.y);
 }
 
 // eight codes times s -> eight bf16
 template <bool E4M3>
 __device__ __forceinline__ uint4 codes_to_bf16(uint2 w, float s) {
-    const uint64_t s2 = pack2(s);
+    const uint64_t s2 = pair(s);
     uint32_t o[4];
     if (E4M3) {
         const uint32_t q[4] = {w.x & 0xffffu, w.x >> 16, w.y & 0xffffu, w.y >> 16};
@@ -114,20 +95,20 @@ __device__ __forceinline__ uint4 codes_to_bf16(uint2 w, float s) {
         for (int i = 0; i < 4; ++i) {
             const __half2 h = __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)q[i], __NV_E4M3));
             const float2 f = __half22float2(h);
-            o[i] = pack_bf16(mul2(pair(f.x, f.y), s2));
+            o[i] = pair_bf16(mul2(pair(f.x, f.y), s2));
         }
         return make_uint4(o[0], o[1], o[2], o[3]);
     }
     // q + 128 in the low byte of 2^23, less 2^23 + 128, times s: exact throughout
     const uint32_t x[2] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u};
-    const uint64_t bias = pack2(-8388736.0f);
+    const uint64_t bias = pair(-8388736.0f);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const uint32_t y = x[i >> 1];
         const int b = 2 * (i & 1);
         const float lo = __uint_as_float(__byte_perm(y, 0x4b000000u, 0x7650 + b));
         const float hi = __uint_as_float(__byte_perm(y, 0x4b000000u, 0x7651 + b));
-        o[i] = pack_bf16(mul2(add2(pair(lo, hi), bias), s2));
+        o[i] = pair_bf16(mul2(add2(pair(lo, hi), bias), s2));
     }
     // a zero byte of x is the code -128, NaN (a borrow may flag the byte above it too)
     const uint32_t z = ((x[0] - 0x01010101u) & ~x[0]) | ((x[1] - 0x01010101u) & ~x[1]);
@@ -309,7 +290,7 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
         for (int kb = kb0; kb < kb1; kb += RGROUP) {
             bool got = true;
             if (lane == 0) got = mbar_wait_inline(lead_full(b), bph, p.status, 44);
-            if (!__shfl_sync(FULL, got ? 1 : 0, 0)) { ok = false; break; }
+            if (!__shfl_sync(FULL_WARP, got ? 1 : 0, 0)) { ok = false; break; }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
             for (int t = 0; t < T; ++t)
@@ -330,7 +311,7 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
         if (ok) {  // every MMA is done: the others' accumulators are whole, the operand ring is free
             bool got = true;
             if (lane == 0) got = mbar_wait_inline(all_done, 0, p.status, 45);
-            ok = __shfl_sync(FULL, got ? 1 : 0, 0) != 0;
+            ok = __shfl_sync(FULL_WARP, got ? 1 : 0, 0) != 0;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         }
         if (ok) {
@@ -396,7 +377,7 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
             if (lane == 0)
                 got = mbar_wait_inline(op_empty(o), oph ^ 1, p.status, 46) &&
                       mbar_wait_inline(raw_full(s), ph, p.status, 47);
-            if (!__shfl_sync(FULL, got ? 1 : 0, 0)) break;
+            if (!__shfl_sync(FULL_WARP, got ? 1 : 0, 0)) break;
             unsigned char* op = smem + o * S::OP;
             const unsigned char* rw = smem + S::RAW_OFF + s * S::RAW;
             uint2 w[RROWS / RPP];
@@ -406,7 +387,7 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
 #pragma unroll
             for (int i = 0; i < RROWS / RPP; ++i) {
                 const int r = i * RPP + lane / LPR;
-                const float sr = __shfl_sync(FULL, sc, RROWS * tile + r);
+                const float sr = __shfl_sync(FULL_WARP, sc, RROWS * tile + r);
                 *reinterpret_cast<uint4*>(op + tile * RA_BYTES + box * 8192 + q8_sw128(r0 + r, unit)) =
                     codes_to_bf16<E4M3>(w[i], sr);
             }

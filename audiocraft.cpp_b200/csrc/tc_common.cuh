@@ -246,23 +246,6 @@ __device__ __forceinline__ void tmem_ld16_wait(uint32_t* r) {
         :: "memory");
 }
 
-// acc (two fp32 in one 64-bit register) += {lo, hi} * {s, s}: two fused multiply-adds, one instruction
-__device__ __forceinline__ void fma2(uint64_t& acc, uint32_t lo, uint32_t hi, uint64_t s2) {
-    uint64_t t;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(t) : "r"(lo), "r"(hi));
-    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(t), "l"(s2));
-}
-__device__ __forceinline__ uint64_t pack2(float v) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %1};" : "=l"(r) : "r"(__float_as_uint(v)));
-    return r;
-}
-__device__ __forceinline__ float2 unpack2(uint64_t v) {
-    uint32_t a, b;
-    asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(v));
-    return make_float2(__uint_as_float(a), __uint_as_float(b));
-}
-
 // ---------------------------------------------------------------------------------------
 // Q8_0 weights dequantised in shared memory on their way into an MMA operand (the 2-CTA GEMM's
 // B and the rank-block kernel's A): a raw slot holds one k-block of biased quants (q + 128) and

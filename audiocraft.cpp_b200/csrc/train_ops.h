@@ -26,7 +26,8 @@ struct OpTensor {
     long ld = 0;
 };
 
-// whether base and stride allow four elements to move as one word
+// whether base and stride allow four elements to move as one word (with columns a multiple of four
+// too, a row's elements all move that way)
 inline bool vec4(const OpTensor& t) {
     return !t.p || (t.ld % 4 == 0 && reinterpret_cast<uintptr_t>(t.p) % (4 * op_bytes(t.type)) == 0);
 }
