@@ -41,14 +41,22 @@ __device__ __forceinline__ Place place(long cols) {
     return p;
 }
 
-// body(place, row, rows, whole) for each of the warp's groups of up to RPW rows
-template <bool VEC, typename Body>
-__device__ __forceinline__ void each_group(long rows, long cols, Body&& body) {
+// body(place, held, row, rows, whole) for each of the warp's groups of up to RPW rows; `held` is what
+// fetch(place, held, row, rows) has loaded of them, one group ahead of its use
+template <bool VEC, typename Held, typename Fetch, typename Body>
+__device__ __forceinline__ void each_group(long rows, long cols, Fetch&& fetch, Body&& body) {
     const Place p = place<VEC>(cols);
-    if (!p.any) return;
+    if (!p.any || p.row >= rows) return;
+    Held next;
     long row = p.row;
-    for (; row + RPW <= rows; row += p.step) body(p, row, RPW, std::true_type());
-    if (row < rows) body(p, row, (int)(rows - row), std::false_type());
+    auto count = [&](long r) { return rows - r < RPW ? (int)(rows - r) : RPW; };
+    fetch(p, next, row, count(row));
+    for (; row + RPW <= rows; row += p.step) {
+        const Held held = next;
+        if (row + p.step < rows) fetch(p, next, row + p.step, count(row + p.step));
+        body(p, held, row, RPW, std::true_type());
+    }
+    if (row < rows) body(p, next, row, count(row), std::false_type());
 }
 
 // the scales of up to RPW rows: lane r holds row r's
@@ -83,16 +91,27 @@ __device__ __forceinline__ void store_rows(const Q8& t, const Place& p, long row
     store_scales(t, p.chunk, row, nr, s);
 }
 
+template <typename T, bool VEC>
+struct HeldRows {
+    Raw4<T, VEC> x[RPW];
+    __device__ __forceinline__ void load(const T* at, long ld, int n, int nr) {
+#pragma unroll
+        for (int r = 0; r < RPW; ++r) x[r].load(at + r * ld, r < nr ? n : 0);
+    }
+};
+
 template <typename T, bool VEC, bool E4M3>
 __global__ void __launch_bounds__(THREADS) store_kernel(const T* x, long ldx, long rows, long cols, Q8 out) {
-    each_group<VEC>(rows, cols, [&](const Place& p, long row, int nr, auto full) {
-        constexpr bool FULL = decltype(full)::value;
-        float v[RPW][4];
-        const T* at = x + row * ldx + p.col;
+    typedef HeldRows<T, VEC> Held;
+    each_group<VEC, Held>(
+        rows, cols,
+        [&](const Place& p, Held& h, long row, int nr) { h.load(x + row * ldx + p.col, ldx, p.n, nr); },
+        [&](const Place& p, const Held& h, long row, int nr, auto whole) {
+            float v[RPW][4];
 #pragma unroll
-        for (int r = 0; r < RPW; ++r) load4<T, VEC>(at + r * ldx, FULL || r < nr ? p.n : 0, v[r]);
-        store_rows<VEC, FULL>(out, p, row, nr, v, E4M3);
-    });
+            for (int r = 0; r < RPW; ++r) h.x[r].values(v[r]);
+            store_rows<VEC, decltype(whole)::value>(out, p, row, nr, v, E4M3);
+        });
 }
 
 // one CTA per 128 x 128 block: a first pass for the maximum, a second that finds the block in L1
@@ -127,85 +146,106 @@ __global__ void __launch_bounds__(THREADS) store_square_kernel(const T* x, long 
     }
 }
 
-// shift: log2 of the block's rows
+template <bool VEC>
+struct HeldCodes {
+    uint32_t w[RPW];
+    float s[RPW];
+    // shift: log2 of the block's rows
+    __device__ __forceinline__ void load(const Q8& t, const Place& p, long row, int nr, int shift) {
+        const uint8_t* q = t.q + row * t.ldq + p.col;
+        const float* scale = t.scale + (long)p.chunk * t.lds;
+#pragma unroll
+        for (int r = 0; r < RPW; ++r) {
+            w[r] = load_codes<VEC>(q + r * t.ldq, r < nr ? p.n : 0);
+            s[r] = r < nr ? scale[(row + r) >> shift] : 0.f;
+        }
+    }
+};
+
 template <typename T, bool VEC, bool E4M3>
 __global__ void __launch_bounds__(THREADS) load_kernel(Q8 in, long rows, long cols, int shift, T* y, long ldy) {
-    each_group<VEC>(rows, cols, [&](const Place& p, long row, int nr, auto full) {
-        constexpr bool FULL = decltype(full)::value;
-        uint32_t w[RPW];
-        float s[RPW];
-        const uint8_t* q = in.q + row * in.ldq + p.col;
-        const float* scale = in.scale + (long)p.chunk * in.lds;
-        T* at = y + row * ldy + p.col;
+    typedef HeldCodes<VEC> Held;
+    each_group<VEC, Held>(
+        rows, cols, [&](const Place& p, Held& h, long row, int nr) { h.load(in, p, row, nr, shift); },
+        [&](const Place& p, const Held& h, long row, int nr, auto whole) {
+            constexpr bool FULL = decltype(whole)::value;
+            T* at = y + row * ldy + p.col;
 #pragma unroll
-        for (int r = 0; r < RPW; ++r) {
-            w[r] = load_codes<VEC>(q + r * in.ldq, FULL || r < nr ? p.n : 0);
-            s[r] = FULL || r < nr ? scale[(row + r) >> shift] : 0.f;
-        }
+            for (int r = 0; r < RPW; ++r) {
+                float v[4];
+                decode4(h.w[r], E4M3, v);
 #pragma unroll
-        for (int r = 0; r < RPW; ++r) {
-            float v[4];
-            decode4(w[r], E4M3, v);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] *= s[r];
-            store4<T, VEC>(at + r * ldy, FULL || r < nr ? p.n : 0, v);
-        }
-    });
+                for (int i = 0; i < 4; ++i) v[i] *= h.s[r];
+                store4<T, VEC>(at + r * ldy, FULL || r < nr ? p.n : 0, v);
+            }
+        });
 }
 
-template <typename T, bool VEC>
+template <typename T, bool VEC, bool E4M3>
 __global__ void __launch_bounds__(THREADS)
     gelu_fwd_kernel(const T* z, long ldz, long rows, long cols, T* g, long ldg, Q8 g8, Q8 z8) {
-    each_group<VEC>(rows, cols, [&](const Place& p, long row, int nr, auto full) {
-        constexpr bool FULL = decltype(full)::value;
-        float v[RPW][4];
-        const T* at = z + row * ldz + p.col;
+    typedef HeldRows<T, VEC> Held;
+    each_group<VEC, Held>(
+        rows, cols,
+        [&](const Place& p, Held& h, long row, int nr) { h.load(z + row * ldz + p.col, ldz, p.n, nr); },
+        [&](const Place& p, const Held& h, long row, int nr, auto whole) {
+            constexpr bool FULL = decltype(whole)::value;
+            float v[RPW][4];
 #pragma unroll
-        for (int r = 0; r < RPW; ++r) load4<T, VEC>(at + r * ldz, FULL || r < nr ? p.n : 0, v[r]);
-        store_rows<VEC, FULL>(z8, p, row, nr, v, z8.e4m3);
+            for (int r = 0; r < RPW; ++r) h.x[r].values(v[r]);
+            store_rows<VEC, FULL>(z8, p, row, nr, v, E4M3);
 #pragma unroll
-        for (int r = 0; r < RPW; ++r)
+            for (int r = 0; r < RPW; ++r) {
+                const uint64_t o[2] = {gelu2(v[r][0], v[r][1]), gelu2(v[r][2], v[r][3])};
+                unpairs(o, v[r]);
+            }
+            if (g) {
+                T* to = g + row * ldg + p.col;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[r][i] = gelu(v[r][i]);
-        if (g) {
-            T* to = g + row * ldg + p.col;
-#pragma unroll
-            for (int r = 0; r < RPW; ++r) store4<T, VEC>(to + r * ldg, FULL || r < nr ? p.n : 0, v[r]);
-        }
-        if (g8.q) store_rows<VEC, FULL>(g8, p, row, nr, v, g8.e4m3);
-    });
+                for (int r = 0; r < RPW; ++r) store4<T, VEC>(to + r * ldg, FULL || r < nr ? p.n : 0, v[r]);
+            }
+            if (g8.q) store_rows<VEC, FULL>(g8, p, row, nr, v, g8.e4m3);
+        });
 }
 
 template <typename T, bool VEC>
+struct HeldBoth {
+    HeldRows<T, VEC> x;
+    HeldCodes<VEC> c;
+};
+
+template <typename T, bool VEC, bool E4M3>
 __global__ void __launch_bounds__(THREADS)
     gelu_bwd_kernel(const T* dg, long lddg, Q8 z8, long rows, long cols, T* dz, long lddz, Q8 dz8) {
-    each_group<VEC>(rows, cols, [&](const Place& p, long row, int nr, auto full) {
-        constexpr bool FULL = decltype(full)::value;
-        float v[RPW][4], s[RPW];
-        uint32_t w[RPW];
-        const T* at = dg + row * lddg + p.col;
-        const uint8_t* q = z8.q + row * z8.ldq + p.col;
-        const float* scale = z8.scale + (long)p.chunk * z8.lds + row;
+    typedef HeldBoth<T, VEC> Held;
+    each_group<VEC, Held>(
+        rows, cols,
+        [&](const Place& p, Held& h, long row, int nr) {
+            h.x.load(dg + row * lddg + p.col, lddg, p.n, nr);
+            h.c.load(z8, p, row, nr, 0);
+        },
+        [&](const Place& p, const Held& h, long row, int nr, auto whole) {
+            constexpr bool FULL = decltype(whole)::value;
+            float v[RPW][4];
 #pragma unroll
-        for (int r = 0; r < RPW; ++r) {
-            load4<T, VEC>(at + r * lddg, FULL || r < nr ? p.n : 0, v[r]);
-            w[r] = load_codes<VEC>(q + r * z8.ldq, FULL || r < nr ? p.n : 0);
-            s[r] = FULL || r < nr ? scale[r] : 0.f;
-        }
+            for (int r = 0; r < RPW; ++r) {
+                float k[4];
+                h.x.x[r].values(v[r]);
+                decode4(h.c.w[r], E4M3, k);
+                uint64_t k2[2], o[2];
+                pairs(k, k2);
+                pairs(v[r], o);
 #pragma unroll
-        for (int r = 0; r < RPW; ++r) {
-            float k[4];
-            decode4(w[r], z8.e4m3, k);
+                for (int i = 0; i < 2; ++i) o[i] = mul2(o[i], gelu_grad2(mul2(k2[i], pair(h.c.s[r]))));
+                unpairs(o, v[r]);
+            }
+            if (dz) {
+                T* to = dz + row * lddz + p.col;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[r][i] *= gelu_grad(k[i] * s[r]);
-        }
-        if (dz) {
-            T* to = dz + row * lddz + p.col;
-#pragma unroll
-            for (int r = 0; r < RPW; ++r) store4<T, VEC>(to + r * lddz, FULL || r < nr ? p.n : 0, v[r]);
-        }
-        if (dz8.q) store_rows<VEC, FULL>(dz8, p, row, nr, v, dz8.e4m3);
-    });
+                for (int r = 0; r < RPW; ++r) store4<T, VEC>(to + r * lddz, FULL || r < nr ? p.n : 0, v[r]);
+            }
+            if (dz8.q) store_rows<VEC, FULL>(dz8, p, row, nr, v, dz8.e4m3);
+        });
 }
 
 // enough warps to fill the GPU (eight CTAs of 256 an SM) or, if there is less, one row group each;
@@ -266,7 +306,8 @@ void gelu_ckpt8_fwd(const OpTensor& z, long rows, long cols, const OpTensor& g, 
     const bool v = cols % 4 == 0 && vec4(z) && vec4(g) && vec4(g8) && vec4(z8);
     by_type(z.type, [&](auto t) {
         typedef decltype(t) T;
-        auto* k = v ? gelu_fwd_kernel<T, true> : gelu_fwd_kernel<T, false>;
+        auto* k = v ? (z8.e4m3 ? gelu_fwd_kernel<T, true, true> : gelu_fwd_kernel<T, true, false>)
+                    : (z8.e4m3 ? gelu_fwd_kernel<T, false, true> : gelu_fwd_kernel<T, false, false>);
         k<<<grid_for(rows, cols), THREADS, 0, s>>>(as<const T>(z), z.ld, rows, cols, as<T>(g), g.ld, g8, z8);
     });
 }
@@ -276,7 +317,8 @@ void gelu_ckpt8_bwd(const OpTensor& dg, const Q8& z8, long rows, long cols, cons
     const bool v = cols % 4 == 0 && vec4(dg) && vec4(dz) && vec4(z8) && vec4(dz8);
     by_type(dg.type, [&](auto t) {
         typedef decltype(t) T;
-        auto* k = v ? gelu_bwd_kernel<T, true> : gelu_bwd_kernel<T, false>;
+        auto* k = v ? (z8.e4m3 ? gelu_bwd_kernel<T, true, true> : gelu_bwd_kernel<T, true, false>)
+                    : (z8.e4m3 ? gelu_bwd_kernel<T, false, true> : gelu_bwd_kernel<T, false, false>);
         k<<<grid_for(rows, cols), THREADS, 0, s>>>(as<const T>(dg), dg.ld, z8, rows, cols, as<T>(dz), dz.ld, dz8);
     });
 }

@@ -220,10 +220,11 @@ __device__ __forceinline__ Top warp_top(const float v[4]) {
 // Four values times 1 / s (exact) -> four codes; with `bad`, what is not finite becomes NaN first.
 // I8: adding 1.5 * 2^23 rounds to nearest even and leaves the whole number in the low byte.
 __device__ __forceinline__ uint32_t encode4(const float v[4], float inv, bool e4m3, bool bad) {
+    const uint64_t i2 = pair(inv);
     if (e4m3) {
         float x[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = v[i] * inv;
+        const uint64_t m[2] = {mul2(pair(v[0], v[1]), i2), mul2(pair(v[2], v[3]), i2)};
+        unpairs(m, x);
         if (bad)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
@@ -233,8 +234,11 @@ __device__ __forceinline__ uint32_t encode4(const float v[4], float inv, bool e4
         return lo | hi << 16;
     }
     uint32_t r[4];
+    float x[4];
+    const uint64_t m[2] = {fma2(pair(v[0], v[1]), i2, pair(12582912.0f)), fma2(pair(v[2], v[3]), i2, pair(12582912.0f))};
+    unpairs(m, x);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = __float_as_uint(fmaf(v[i], inv, 12582912.0f));
+    for (int i = 0; i < 4; ++i) r[i] = __float_as_uint(x[i]);
     if (bad)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -299,27 +303,52 @@ __device__ __forceinline__ uint32_t store_block(uint8_t* p, int n, const float v
 // the polynomial of degree 8 fitted (iteratively reweighted least squares, relative error
 // 5.8e-8 for |z| <= 14.5, where Q leaves fp32's range) to exp(z^2 / 2) (1 - Phi(|z|)).  The form
 // keeps relative accuracy in the tail, where 1 - erf would cancel.  With the hardware's
-// reciprocal and exponential the results are within about 1e-6 of gelu and gelu'.
-__device__ __forceinline__ float normal_tail(float a, float e) {
-    const float t = __fdividef(1.0f, fmaf(0.3f, a, 1.0f));
-    float r = 0.03840748965740204f;
-    r = fmaf(r, t, -0.1693079173564911f);
-    r = fmaf(r, t, 0.22895267605781555f);
-    r = fmaf(r, t, -0.07684063166379929f);
-    r = fmaf(r, t, 0.14276590943336487f);
-    r = fmaf(r, t, 0.0945856124162674f);
-    r = fmaf(r, t, 0.121945321559906f);
-    r = fmaf(r, t, 0.11948420107364655f);
-    r = fmaf(r, t, 7.372795153059997e-06f);
-    return r * e;
+// reciprocal and exponential (which flushes below 2^-126) the results are within about 1e-6 of
+// gelu and gelu'.  Two values at a time: these passes are bound by issued instructions.
+__device__ __forceinline__ float ex2(float v) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
 }
-__device__ __forceinline__ float gelu(float z) {
-    const float a = fabsf(z), q = normal_tail(a, __expf(-0.5f * a * a));
-    return z * (z > 0.f ? 1.0f - q : q);
+__device__ __forceinline__ float rcp(float v) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
 }
-__device__ __forceinline__ float gelu_grad(float z) {
-    const float a = fabsf(z), e = __expf(-0.5f * a * a), q = normal_tail(a, e);
-    return fmaf(z * 0.3989422804014327f, e, z > 0.f ? 1.0f - q : q);
+// Q and exp(-z^2 / 2) of a = min(|z|, 16): beyond 16 both are 0
+__device__ __forceinline__ void normal_tail(uint64_t a, uint64_t& q, uint64_t& e) {
+    const float2 x = unpair(mul2(mul2(a, a), pair(-0.72134752044448170f)));  // -z^2 / 2 in powers of two
+    const float2 d = unpair(fma2(a, pair(0.3f), pair(1.0f)));
+    const uint64_t t = pair(rcp(d.x), rcp(d.y));
+    e = pair(ex2(x.x), ex2(x.y));
+    uint64_t r = pair(0.03840748965740204f);
+    r = fma2(r, t, pair(-0.1693079173564911f));
+    r = fma2(r, t, pair(0.22895267605781555f));
+    r = fma2(r, t, pair(-0.07684063166379929f));
+    r = fma2(r, t, pair(0.14276590943336487f));
+    r = fma2(r, t, pair(0.0945856124162674f));
+    r = fma2(r, t, pair(0.121945321559906f));
+    r = fma2(r, t, pair(0.11948420107364655f));
+    r = fma2(r, t, pair(7.372795153059997e-06f));
+    q = mul2(r, e);
+}
+// z Phi(z) = max(z, 0) - |z| Q
+__device__ __forceinline__ uint64_t gelu2(float z0, float z1) {
+    const uint64_t a = pair(fminf(fabsf(z0), 16.f), fminf(fabsf(z1), 16.f));
+    uint64_t q, e;
+    normal_tail(a, q, e);
+    return fma2(mul2(a, pair(-1.0f)), q, pair(max_nan(z0, 0.f), max_nan(z1, 0.f)));
+}
+// Phi(z) + z phi(z), Phi(z) = [z > 0] - sign(z) Q
+__device__ __forceinline__ uint64_t gelu_grad2(uint64_t z) {
+    const float2 f = unpair(z);
+    const uint64_t a = pair(fminf(fabsf(f.x), 16.f), fminf(fabsf(f.y), 16.f));
+    uint64_t q, e;
+    normal_tail(a, q, e);
+    const float2 u = unpair(q);
+    const uint64_t sq = pair(f.x > 0.f ? -u.x : u.x, f.y > 0.f ? -u.y : u.y);
+    const uint64_t step = pair(f.x > 0.f ? 1.f : 0.f, f.y > 0.f ? 1.f : 0.f);
+    return fma2(mul2(z, pair(0.3989422804014327f)), e, add2(step, sq));
 }
 
 }  // namespace c8
