@@ -35,17 +35,17 @@ constexpr int BM = 128, BK = 128;
 constexpr int A_BYTES = BM * BK;
 constexpr int NTHREADS = 384;  // four warps that feed, eight that add
 constexpr int ADDERS = 8;
-constexpr int EPI_LD = 36;     // floats per staged row of 32: 16-byte accesses of 8 lanes hit all banks
-constexpr int EPI_BYTES = 32 * EPI_LD * 4;  // per adding warp
+constexpr int AHEAD = 8;       // k-blocks whose scales an adding thread has under way
+constexpr int SCALE_BYTES = AHEAD * ADDERS * 32 * 8;
 
+// BN: columns of a tile
 template <int BN>
 struct Shape {
-    static constexpr int B_BYTES = BN * BK;
-    static constexpr int STAGE = A_BYTES + B_BYTES;
-    static constexpr int STAGES = BN == 256 ? 3 : 5;
+    static constexpr int STAGE = A_BYTES + BN * BK;
+    static constexpr int STAGES = BN == 256 ? 4 : 6;
     static constexpr int HALF = BN / 2;  // columns of an adding warp
-    static constexpr int EPI_OFF = STAGES * STAGE;
-    static constexpr int BAR_OFF = EPI_OFF + ADDERS * EPI_BYTES;
+    static constexpr int SCALE_OFF = STAGES * STAGE;
+    static constexpr int BAR_OFF = SCALE_OFF + SCALE_BYTES;
     static constexpr int SMEM = BAR_OFF + 8 * (2 * STAGES + 5) + 16 + 1024 /*align*/;
     static constexpr int TMEM = 2 * BN;
 };
@@ -57,14 +57,15 @@ struct Maps {
 struct Params {
     long M, N, K;
     int nk;           // k-blocks
-    long mt, nt;      // tiles
+    int mt, nt;       // tiles
+    int dm, dn;       // the grid's stride over them
     const float *sx, *sw;
     long ldsx, ldsw;
     const float* bias;
     void* y;
     int y_type, accumulate;
     long ldy;
-    int vec;          // rows of y move four elements at a time
+    int vec;          // rows of y move in whole sectors, bias four at a time
     int* status;
 };
 
@@ -79,30 +80,92 @@ __device__ __forceinline__ void put_value(const Params& p, long at, float v) {
     else static_cast<__nv_bfloat16*>(p.y)[at] = from_f32<__nv_bfloat16>(v);
 }
 
-// four columns n .. n + 3 of row m: bias, old value, one rounding
-__device__ __forceinline__ void put4(const Params& p, long m, long n, float4 f) {
-    float v[4] = {f.x, f.y, f.z, f.w};
-    const long at = m * p.ldy + n;
-    const int left = p.N - n < 4 ? (int)(p.N - n) : 4;
-    if (p.bias)
+// a whole 32-byte sector in one access
+__device__ __forceinline__ void store_sector(void* p, const uint32_t w[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                 "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
+__device__ __forceinline__ void load_sector(const void* p, uint32_t w[8]) {
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                 : "l"(p)
+                 : "memory");
+}
+
+// 16 columns n .. n + 15 of a row: bias, old value, one rounding; at counts elements of y.  Whole
+// groups of aligned rows move as 32-byte sectors (a thread's neighbours hold other rows).
+__device__ __forceinline__ void put16(const Params& p, long at, long n, float v[16]) {
+    const int left = p.N - n < 16 ? (int)(p.N - n) : 16;
+    if (left <= 0) return;
+    if (p.bias) {
+        if (left == 16 && p.vec)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (i < left) v[i] += p.bias[n + i];
-    if (p.vec && left == 4) {
-        char* y = static_cast<char*>(p.y) + at * (p.y_type == OP_F32 ? 4 : 2);
-        if (p.accumulate) {
-            float o[4];
-            if (p.y_type == OP_F32) load4_bytes<4, true>(y, false, 4, o);
-            else load4_bytes<2, true>(y, p.y_type == OP_F16, 4, o);
+            for (int i = 0; i < 16; i += 4) {
+                const float4 b = __ldg(reinterpret_cast<const float4*>(p.bias + n + i));
+                v[i] += b.x; v[i + 1] += b.y; v[i + 2] += b.z; v[i + 3] += b.w;
+            }
+        else
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] += o[i];
-        }
-        if (p.y_type == OP_F32) store4_bytes<4, true>(y, false, 4, v);
-        else store4_bytes<2, true>(y, p.y_type == OP_F16, 4, v);
+            for (int i = 0; i < 16; ++i)
+                if (i < left) v[i] += __ldg(p.bias + n + i);
+    }
+    if (left < 16 || !p.vec) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (i < left) put_value(p, at + i, p.accumulate ? old_value(p, at + i) + v[i] : v[i]);
         return;
     }
-    for (int i = 0; i < left; ++i) put_value(p, at + i, p.accumulate ? old_value(p, at + i) + v[i] : v[i]);
+    if (p.y_type == OP_F32) {
+        float* y = static_cast<float*>(p.y) + at;
+#pragma unroll
+        for (int h = 0; h < 16; h += 8) {
+            if (p.accumulate) {
+                uint32_t o[8];
+                load_sector(y + h, o);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[h + i] += __uint_as_float(o[i]);
+            }
+            uint32_t w[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(v[h + i]);
+            store_sector(y + h, w);
+        }
+        return;
+    }
+    uint16_t* y = static_cast<uint16_t*>(p.y) + at;
+    const bool half = p.y_type == OP_F16;
+    uint32_t w[8];
+    if (p.accumulate) {
+        load_sector(y, w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float2 f = half ? unpack_f16(w[i])
+                                  : make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+            v[2 * i] += f.x;
+            v[2 * i + 1] += f.y;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        w[i] = half ? pack_f16(v[2 * i], v[2 * i + 1]) : pack_bf16(v[2 * i], v[2 * i + 1]);
+    store_sector(y, w);
 }
+
+// the tiles of one CTA, column tiles first: CTAs that run together share rows of X
+struct Walk {
+    int m, n;
+    __device__ __forceinline__ explicit Walk(const Params& p) : m(blockIdx.x / p.nt), n(blockIdx.x % p.nt) {}
+    __device__ __forceinline__ bool any(const Params& p) const { return m < p.mt; }
+    __device__ __forceinline__ void next(const Params& p) {
+        m += p.dm;
+        n += p.dn;
+        if (n >= p.nt) {
+            n -= p.nt;
+            ++m;
+        }
+    }
+};
 
 template <int BN, bool MN>
 __global__ void __launch_bounds__(NTHREADS, 1) gemm_f8_kernel(const __grid_constant__ Maps maps, const Params p) {
@@ -144,7 +207,6 @@ __global__ void __launch_bounds__(NTHREADS, 1) gemm_f8_kernel(const __grid_const
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *tmem_slot;
-    const long tiles = p.mt * p.nt;
 
     // Registers: the four feeding warps give theirs to the eight that hold the sums (launched with
     // 168 each: 128 * 56 + 256 * 224 = 384 * 168).
@@ -156,8 +218,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) gemm_f8_kernel(const __grid_const
             uint32_t ph = 0;
             long issued = 0;
             bool ok = true;
-            for (long tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
-                const int m0 = (int)(tile / p.nt * BM), n0 = (int)(tile % p.nt * BN);
+            for (Walk t(p); ok && t.any(p); t.next(p)) {
+                const int m0 = t.m * BM, n0 = t.n * BN;
                 for (int kb = 0; kb < p.nk; ++kb, ++issued) {
                     if (!mbar_wait_inline(empty_bar(s), ph ^ 1, p.status, 31)) { ok = false; break; }
                     const uint32_t sa = base + s * S::STAGE, sb = sa + A_BYTES;
@@ -189,9 +251,10 @@ __global__ void __launch_bounds__(NTHREADS, 1) gemm_f8_kernel(const __grid_const
             int s = 0, b = 0;
             uint32_t ph = 0, bph = 0;
             bool ok = true;
-            for (long tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
+            for (Walk t(p); ok && t.any(p); t.next(p)) {
                 for (int kb = 0; kb < p.nk; ++kb) {
-                    if (!mbar_wait_inline(tempty(b), bph ^ 1, p.status, 32) || !mbar_wait_inline(full_bar(s), ph, p.status, 33)) {
+                    if (!mbar_wait_inline(tempty(b), bph ^ 1, p.status, 32) ||
+                        !mbar_wait_inline(full_bar(s), ph, p.status, 33)) {
                         ok = false;
                         break;
                     }
@@ -217,27 +280,52 @@ __global__ void __launch_bounds__(NTHREADS, 1) gemm_f8_kernel(const __grid_const
         asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         const int quad = warp & 3, half = (warp - 4) >> 2;
         const uint32_t tcol = tmem + ((uint32_t)(quad * 32) << 16) + half * S::HALF;
-        float* stage = reinterpret_cast<float*>(smem + S::EPI_OFF + (warp - 4) * EPI_BYTES);
+        // The scales of a k-block are needed every few hundred cycles and mostly come from HBM: each thread
+        // copies its own row's and its columns' AHEAD blocks ahead (also into the next tile).
+        const int slot0 = (warp - 4) * 32 + lane;
+        float2* const ring = reinterpret_cast<float2*>(smem + S::SCALE_OFF);
+        // W's scales: [k-block][n-block], or [n-block][k-block] of a weight stored [K][N]
+        const long wstep = MN ? 1 : p.ldsw;
+        Walk coming(p);
+        int ckb = 0, cslot = 0;
+        const float *csx = p.sx, *csw = p.sw;
+        auto ahead = [&]() {
+            if (coming.any(p)) {
+                if (ckb == 0) {
+                    const long m = (long)coming.m * BM + quad * 32 + lane;
+                    const long n = (long)coming.n * BN + half * S::HALF;
+                    csx = p.sx + (m < p.M ? m : 0);
+                    csw = p.sw + (n < p.N ? (MN ? n / 128 * p.ldsw : n / 128) : 0);
+                }
+                const uint32_t to = smem_u32(ring + cslot * (ADDERS * 32) + slot0);
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(csx) : "memory");
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + 4), "l"(csw) : "memory");
+                csx += p.ldsx;
+                csw += wstep;
+                if (++ckb == p.nk) {
+                    ckb = 0;
+                    coming.next(p);
+                }
+            }
+            cp_async_commit();
+            if (++cslot == AHEAD) cslot = 0;
+        };
+        for (int i = 0; i < AHEAD - 1; ++i) ahead();
+        int slot = 0;
         int b = 0;
         uint32_t bph = 0;
         bool ok = true;
-        for (long tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
-            const long m0 = tile / p.nt * BM + quad * 32, n0 = tile % p.nt * BN + half * S::HALF;
-            const long m = m0 + lane, nb = n0 / 128;
-            const float* sx = p.sx + (m < p.M ? m : 0);
-            // W's scales: [k-block][n-block], or [n-block][k-block] of a weight stored [K][N]
-            const float* sw = p.sw + (n0 < p.N ? (MN ? nb * p.ldsw : nb) : 0);
-            const long wstep = MN ? 1 : p.ldsw;
+        for (Walk w(p); ok && w.any(p); w.next(p)) {
+            const long m0 = (long)w.m * BM + quad * 32, n0 = (long)w.n * BN + half * S::HALF;
             uint64_t acc[S::HALF / 2];
 #pragma unroll
             for (int i = 0; i < S::HALF / 2; ++i) acc[i] = 0;
-            float a = sx[0], w = sw[0];
             for (int kb = 0; kb < p.nk; ++kb) {
-                const uint64_t sc = pair(a * w);
-                if (kb + 1 < p.nk) {
-                    a = sx[(long)(kb + 1) * p.ldsx];
-                    w = sw[(long)(kb + 1) * wstep];
-                }
+                ahead();
+                cp_async_wait<AHEAD - 1>();
+                const float2 sw = ring[slot * (ADDERS * 32) + slot0];
+                const uint64_t sc = pair(sw.x * sw.y);
+                if (++slot == AHEAD) slot = 0;
                 bool got = true;
                 if (lane == 0) got = mbar_wait_inline(tfull(b), bph, p.status, 34);
                 if (!__shfl_sync(FULL_WARP, got ? 1 : 0, 0)) { ok = false; break; }
@@ -261,26 +349,23 @@ __global__ void __launch_bounds__(NTHREADS, 1) gemm_f8_kernel(const __grid_const
                 if (b == 0) bph ^= 1;
             }
             if (!ok) break;
-            // epilogue: 32 x 32 at a time, a row per lane in, four rows of 128 bytes per access out
+            // epilogue: a row per thread, 16 columns at a time
+            const long m = m0 + lane;
+            if (m < p.M) {
 #pragma unroll
-            for (int c = 0; c < S::HALF / 32; ++c) {
-                if (n0 + 32 * c >= p.N) break;
-                __syncwarp();
+                for (int c = 0; c < S::HALF / 16; ++c) {
+                    float v[16];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float2 u = unpair(acc[16 * c + 2 * i]), v = unpair(acc[16 * c + 2 * i + 1]);
-                    *reinterpret_cast<float4*>(stage + lane * EPI_LD + 4 * i) = make_float4(u.x, u.y, v.x, v.y);
-                }
-                __syncwarp();
-#pragma unroll 1
-                for (int i = 0; i < 8; ++i) {
-                    const int r = 4 * i + (lane >> 3);
-                    const long n = n0 + 32 * c + 4 * (lane & 7);
-                    const float4 f = *reinterpret_cast<const float4*>(stage + r * EPI_LD + 4 * (lane & 7));
-                    if (m0 + r < p.M && n < p.N) put4(p, m0 + r, n, f);
+                    for (int i = 0; i < 8; ++i) {
+                        const float2 f = unpair(acc[8 * c + i]);
+                        v[2 * i] = f.x;
+                        v[2 * i + 1] = f.y;
+                    }
+                    put16(p, m * p.ldy + n0 + 16 * c, n0 + 16 * c, v);
                 }
             }
         }
+        cp_async_wait<0>();
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
@@ -385,10 +470,19 @@ void launch(const GemmF8& a, Params p, cudaStream_t s) {
     tc_make_map_u8(&maps.x, a.x.q, a.M, a.K, a.x.ldq, BK, BM);
     if (MN) tc_make_map_u8(&maps.w, a.w.q, a.K, a.N, a.w.ldq, 128, BK);
     else tc_make_map_u8(&maps.w, a.w.q, a.N, a.K, a.w.ldq, BK, BN);
-    p.mt = (a.M + BM - 1) / BM;
-    p.nt = (a.N + BN - 1) / BN;
-    const long tiles = p.mt * p.nt, sms = current_sm_count();
-    gemm_f8_kernel<BN, MN><<<(unsigned)(tiles < sms ? tiles : sms), NTHREADS, S::SMEM, s>>>(maps, p);
+    p.mt = (int)((a.M + BM - 1) / BM);
+    p.nt = (int)((a.N + BN - 1) / BN);
+    const long tiles = (long)p.mt * p.nt, sms = current_sm_count();
+    const int ctas = (int)(tiles < sms ? tiles : sms);
+    p.dm = ctas / p.nt;
+    p.dn = ctas % p.nt;
+    gemm_f8_kernel<BN, MN><<<(unsigned)ctas, NTHREADS, S::SMEM, s>>>(maps, p);
+}
+
+template <int BN>
+void launch(const GemmF8& a, const Params& p, cudaStream_t s) {
+    if (a.w_mn) launch<BN, true>(a, p, s);
+    else launch<BN, false>(a, p, s);
 }
 
 }  // namespace
@@ -398,8 +492,8 @@ void gemm_f8(const GemmF8& a, cudaStream_t s) {
     p.M = a.M; p.N = a.N; p.K = a.K; p.nk = (int)((a.K + BK - 1) / BK);
     p.sx = a.x.scale; p.sw = a.w.scale; p.ldsx = a.x.lds; p.ldsw = a.w.lds;
     p.bias = a.bias; p.y = const_cast<void*>(a.y.p); p.y_type = a.y.type; p.accumulate = a.accumulate ? 1 : 0;
-    p.ldy = a.y.ld; p.vec = vec4(a.y) ? 1 : 0; p.status = a.status;
-    p.mt = p.nt = 0;
+    p.ldy = a.y.ld; p.vec = a.y.ld * op_bytes(a.y.type) % 32 == 0 && reinterpret_cast<uintptr_t>(a.y.p) % 32 == 0 && vec4(a.bias); p.status = a.status;
+    p.mt = p.nt = p.dm = p.dn = 0;
     if (a.M <= SM_MAX_M && !a.w_mn) {
         const unsigned ctas = (unsigned)((a.N + SM_ROWS - 1) / SM_ROWS);
         if (a.M <= 8) gemm_f8_small_kernel<1><<<ctas, SM_WARPS * 32, 0, s>>>(a.x.q, a.x.ldq, a.w.q, a.w.ldq, p);
@@ -409,8 +503,8 @@ void gemm_f8(const GemmF8& a, cudaStream_t s) {
     // 256-wide tiles unless 128-wide ones finish in fewer column-rounds over the SMs
     const long mt = (a.M + BM - 1) / BM, sms = current_sm_count();
     auto cost = [&](long bn) { return (mt * ((a.N + bn - 1) / bn) + sms - 1) / sms * bn; };
-    if (cost(128) < cost(256)) a.w_mn ? launch<128, true>(a, p, s) : launch<128, false>(a, p, s);
-    else a.w_mn ? launch<256, true>(a, p, s) : launch<256, false>(a, p, s);
+    if (cost(128) < cost(256)) launch<128>(a, p, s);
+    else launch<256>(a, p, s);
 }
 
 }  // namespace act
