@@ -35,8 +35,12 @@ constexpr int BM = 128, BK = 128;
 constexpr int A_BYTES = BM * BK;
 constexpr int NTHREADS = 384;  // four warps that feed, eight that add
 constexpr int ADDERS = 8;
-constexpr int AHEAD = 8;       // k-blocks whose scales an adding thread has under way
-constexpr int SCALE_BYTES = AHEAD * ADDERS * 32 * 8;
+// Scales of a k-block (128 of X, two of W) lie in a ring of their own: a slot is written when its
+// stage is, at most STAGES blocks ahead of the MMAs, and read at most two blocks (the TMEM
+// buffers) behind them, so that it is not overwritten before STAGES + 2 blocks have passed.
+constexpr int SCALE_SLOTS = 8;
+constexpr int SCALE_LD = BM + 4;  // floats
+constexpr int SCALE_BYTES = SCALE_SLOTS * SCALE_LD * 4;
 
 // BN: columns of a tile
 template <int BN>
@@ -48,6 +52,7 @@ struct Shape {
     static constexpr int BAR_OFF = SCALE_OFF + SCALE_BYTES;
     static constexpr int SMEM = BAR_OFF + 8 * (2 * STAGES + 5) + 16 + 1024 /*align*/;
     static constexpr int TMEM = 2 * BN;
+    static_assert(STAGES + 2 <= SCALE_SLOTS, "a scale would be overwritten before it is read");
 };
 
 struct Maps {
@@ -61,6 +66,7 @@ struct Params {
     int dm, dn;       // the grid's stride over them
     const float *sx, *sw;
     long ldsx, ldsw;
+    int sx_vec;       // X's scales move four at a time
     const float* bias;
     void* y;
     int y_type, accumulate;
@@ -187,7 +193,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) gemm_f8_kernel(const __grid_const
         prefetch_tmap(&maps.x);
         prefetch_tmap(&maps.w);
         for (int s = 0; s < S::STAGES; ++s) {
-            mbar_init(full_bar(s), 1);
+            mbar_init(full_bar(s), 1 + 32);  // the tiles' bytes and the lanes that copy the scales
             mbar_init(empty_bar(s), 1);
         }
         for (int b = 0; b < 2; ++b) {
@@ -240,6 +246,42 @@ __global__ void __launch_bounds__(NTHREADS, 1) gemm_f8_kernel(const __grid_const
                     const long i = issued - 1 - j;
                     mbar_drain_inline(full_bar((int)(i % S::STAGES)), (uint32_t)((i / S::STAGES) & 1));
                 }
+        } else if (warp == 2) {
+            // -------------------------------------------------------- scales
+            int s = 0, slot = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            const uint32_t ring = base + S::SCALE_OFF;
+            for (Walk t(p); ok && t.any(p); t.next(p)) {
+                // rows 4 lane .. 4 lane + 3 of X, and (lanes 0, 1) 128 columns of W each
+                const long m = (long)t.m * BM + 4 * lane, n = (long)t.n * BN + 128 * lane;
+                const bool whole = p.sx_vec && m + 4 <= p.M, w = lane < BN / 128 && n < p.N;
+                const float* sx = p.sx + m;
+                // W's scales: [k-block][n-block], or [n-block][k-block] of a weight stored [K][N]
+                const float* sw = p.sw + (w ? (MN ? n / 128 * p.ldsw : n / 128) : 0);
+                for (int kb = 0; kb < p.nk; ++kb) {
+                    bool got = true;
+                    if (lane == 0) got = mbar_wait_inline(empty_bar(s), ph ^ 1, p.status, 35);
+                    if (!__shfl_sync(FULL_WARP, got ? 1 : 0, 0)) { ok = false; break; }
+                    const uint32_t to = ring + slot * SCALE_LD * 4;
+                    if (whole) {
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + 16 * lane), "l"(sx) : "memory");
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (m + i < p.M)
+                                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + 16 * lane + 4 * i),
+                                             "l"(sx + i) : "memory");
+                    }
+                    if (w) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + 4 * (BM + lane)), "l"(sw) : "memory");
+                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(full_bar(s)) : "memory");
+                    sx += p.ldsx;
+                    sw += MN ? 1 : p.ldsw;
+                    if (++slot == SCALE_SLOTS) slot = 0;
+                    if (++s == S::STAGES) { s = 0; ph ^= 1; }
+                }
+            }
+            cp_async_wait_all();
         } else if (warp == 1 && lane == 0) {
             // -------------------------------------------------------- MMA
             // fp32 accumulator (bit 4), E4M3 operands (0), B's major, N >> 3, M >> 4
@@ -280,37 +322,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) gemm_f8_kernel(const __grid_const
         asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         const int quad = warp & 3, half = (warp - 4) >> 2;
         const uint32_t tcol = tmem + ((uint32_t)(quad * 32) << 16) + half * S::HALF;
-        // The scales of a k-block are needed every few hundred cycles and mostly come from HBM: each thread
-        // copies its own row's and its columns' AHEAD blocks ahead (also into the next tile).
-        const int slot0 = (warp - 4) * 32 + lane;
-        float2* const ring = reinterpret_cast<float2*>(smem + S::SCALE_OFF);
-        // W's scales: [k-block][n-block], or [n-block][k-block] of a weight stored [K][N]
-        const long wstep = MN ? 1 : p.ldsw;
-        Walk coming(p);
-        int ckb = 0, cslot = 0;
-        const float *csx = p.sx, *csw = p.sw;
-        auto ahead = [&]() {
-            if (coming.any(p)) {
-                if (ckb == 0) {
-                    const long m = (long)coming.m * BM + quad * 32 + lane;
-                    const long n = (long)coming.n * BN + half * S::HALF;
-                    csx = p.sx + (m < p.M ? m : 0);
-                    csw = p.sw + (n < p.N ? (MN ? n / 128 * p.ldsw : n / 128) : 0);
-                }
-                const uint32_t to = smem_u32(ring + cslot * (ADDERS * 32) + slot0);
-                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(csx) : "memory");
-                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + 4), "l"(csw) : "memory");
-                csx += p.ldsx;
-                csw += wstep;
-                if (++ckb == p.nk) {
-                    ckb = 0;
-                    coming.next(p);
-                }
-            }
-            cp_async_commit();
-            if (++cslot == AHEAD) cslot = 0;
-        };
-        for (int i = 0; i < AHEAD - 1; ++i) ahead();
+        const float* const scales = reinterpret_cast<const float*>(smem + S::SCALE_OFF);
         int slot = 0;
         int b = 0;
         uint32_t bph = 0;
@@ -321,15 +333,13 @@ __global__ void __launch_bounds__(NTHREADS, 1) gemm_f8_kernel(const __grid_const
 #pragma unroll
             for (int i = 0; i < S::HALF / 2; ++i) acc[i] = 0;
             for (int kb = 0; kb < p.nk; ++kb) {
-                ahead();
-                cp_async_wait<AHEAD - 1>();
-                const float2 sw = ring[slot * (ADDERS * 32) + slot0];
-                const uint64_t sc = pair(sw.x * sw.y);
-                if (++slot == AHEAD) slot = 0;
                 bool got = true;
                 if (lane == 0) got = mbar_wait_inline(tfull(b), bph, p.status, 34);
                 if (!__shfl_sync(FULL_WARP, got ? 1 : 0, 0)) { ok = false; break; }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const float* at = scales + slot * SCALE_LD;
+                const uint64_t sc = pair(at[quad * 32 + lane] * at[BM + (BN == 256 ? half : 0)]);
+                if (++slot == SCALE_SLOTS) slot = 0;
                 uint32_t r[2][16];
                 tmem_ld16_start(tcol + b * BN, r[0]);
 #pragma unroll
@@ -365,7 +375,6 @@ __global__ void __launch_bounds__(NTHREADS, 1) gemm_f8_kernel(const __grid_const
                 }
             }
         }
-        cp_async_wait<0>();
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
@@ -491,6 +500,7 @@ void gemm_f8(const GemmF8& a, cudaStream_t s) {
     Params p;
     p.M = a.M; p.N = a.N; p.K = a.K; p.nk = (int)((a.K + BK - 1) / BK);
     p.sx = a.x.scale; p.sw = a.w.scale; p.ldsx = a.x.lds; p.ldsw = a.w.lds;
+    p.sx_vec = vec4(a.x.scale) && a.x.lds % 4 == 0;
     p.bias = a.bias; p.y = const_cast<void*>(a.y.p); p.y_type = a.y.type; p.accumulate = a.accumulate ? 1 : 0;
     p.ldy = a.y.ld; p.vec = a.y.ld * op_bytes(a.y.type) % 32 == 0 && reinterpret_cast<uintptr_t>(a.y.p) % 32 == 0 && vec4(a.bias); p.status = a.status;
     p.mt = p.nt = p.dm = p.dn = 0;
