@@ -19,6 +19,8 @@
 #include <cuda.h>
 
 #include <atomic>
+#include <cstring>
+#include <type_traits>
 
 #include "ckpt8.cuh"
 #include "tc_common.cuh"
@@ -61,7 +63,7 @@ struct RParams {
     int rows, nk, nb, nbp;  // nbp: nb rounded up to 16
     long cols;
     const void* u;
-    int u_type, u_vec, pieces;
+    int u_vec;
     long ldu;
     const float* scale;
     long lds;
@@ -75,9 +77,6 @@ struct RParams {
 struct RMaps {
     CUtensorMap x;
 };
-
-__device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
-__device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
 __device__ __forceinline__ uint32_t pair_bf16(uint64_t v) {
     const float2 f = unpair(v);
@@ -119,48 +118,40 @@ __device__ __forceinline__ uint4 codes_to_bf16(uint2 w, float s) {
     return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
-// eight values of row t of U from column j on; missing rows and columns are 0
-__device__ __forceinline__ void load_u(const RParams& p, long t, int j, float v[8]) {
-    const bool in = t < p.rows;
-    const long at = t * p.ldu + j;
-    if (in && p.u_vec && j + 8 <= p.nb) {
-        if (p.u_type == OP_F32) {
-            const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(p.u) + at);
-            const float4 b = *reinterpret_cast<const float4*>(static_cast<const float*>(p.u) + at + 4);
-            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-            v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-        } else {
-            const uint2 a = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.u) + at);
-            const uint2 b = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.u) + at + 4);
-            const uint32_t w[4] = {a.x, a.y, b.x, b.y};
+// Eight neighbouring values of a row of U as they lie in memory: as words where base, stride and
+// nb allow, else one by one; `have` counts the columns from the first one (0: none), missing
+// ones are 0.
+template <typename U>
+struct UnitOfU {
+    static constexpr int WORDS = 8 * sizeof(U) / 8;  // 8-byte words
+    uint2 w[WORDS];
+    __device__ __forceinline__ void load(const U* at, int have, bool vec) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float2 f = p.u_type == OP_F16 ? unpack_f16(w[i]) : make_float2(bf16_lo(w[i]), bf16_hi(w[i]));
-                v[2 * i] = f.x;
-                v[2 * i + 1] = f.y;
-            }
+        for (int i = 0; i < WORDS; ++i) w[i] = make_uint2(0, 0);
+        if (vec) {
+            if (have > 0)  // nb is a multiple of eight here: all or nothing
+#pragma unroll
+                for (int i = 0; i < WORDS; ++i) w[i] = reinterpret_cast<const uint2*>(at)[i];
+            return;
         }
-        return;
-    }
+        U e[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        v[i] = 0.f;
-        if (in && j + i < p.nb)
-            v[i] = p.u_type == OP_F32   ? static_cast<const float*>(p.u)[at + i]
-                   : p.u_type == OP_F16 ? to_f32(static_cast<const f16*>(p.u)[at + i])
-                                        : to_f32(static_cast<const __nv_bfloat16*>(p.u)[at + i]);
+        for (int i = 0; i < 8; ++i) e[i] = i < have ? at[i] : U(0.f);
+        memcpy(w, e, sizeof(e));
     }
-}
+    __device__ __forceinline__ void values(float v[8]) const {
+        U e[8];
+        memcpy(e, w, sizeof(e));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = to_f32(e[i]);
+    }
+};
 
-// The next bf16 piece of v is its upper half-word (cut off, not rounded: three pieces hold all 24 bits
-// and none can overflow); what is left of v is exact.  An infinity is all in its first piece.
-__device__ __forceinline__ float left_of(float v) {
-    return abs_bits(v) == 0x7f800000u ? 0.f : v - __uint_as_float(__float_as_uint(v) & 0xffff0000u);
-}
-
-template <int T, bool E4M3>
+// U: type of U; PIECES bf16 pieces hold all of it
+template <int T, bool E4M3, typename U>
 __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant__ RMaps maps, const RParams p) {
     typedef RShape<T> S;
+    constexpr int PIECES = sizeof(U) == 4 ? 3 : std::is_same<U, f16>::value ? 2 : 1;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t base = (raw + 1023) & ~1023u;
@@ -233,7 +224,7 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
             // fp32 accumulator, bf16 operands (1), both MN-major, N >> 3, M >> 4
             const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (1u << 16) | (8u << 24);
             const uint32_t lead_desc = idesc | ((uint32_t)(p.nbp >> 3) << 17);
-            const uint32_t other_desc = idesc | ((uint32_t)(((p.pieces - 1) * p.nbp) >> 3) << 17);
+            const uint32_t other_desc = idesc | ((uint32_t)(((PIECES - 1) * p.nbp) >> 3) << 17);
             const uint64_t a_desc = smem_desc(base, 8192, 1024);
             const uint64_t b_desc = smem_desc(base + T * RA_BYTES, 8192, 1024);
             constexpr uint32_t step = 2048 >> 4;  // 16 rows of 128 bytes
@@ -253,7 +244,7 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
                     for (int k = 0; k < RK / 16; ++k)
                         mma_f16(tmem + (b * T + t) * 64, a + step * k, bb + step * k, lead_desc,
                                 (in_group > 0 || k > 0) ? 1u : 0u);
-                    if (p.pieces > 1)
+                    if (PIECES > 1)
 #pragma unroll
                         for (int k = 0; k < RK / 16; ++k)
                             mma_f16(tmem + S::OTHER + t * 128, a + step * k, bb + (RB_BOX >> 4) + step * k, other_desc,
@@ -318,7 +309,7 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
             float* part = reinterpret_cast<float*>(smem);
 #pragma unroll
             for (int t = 0; t < T; ++t) {
-                for (int q = p.pieces - 1; q > 0; --q)
+                for (int q = PIECES - 1; q > 0; --q)
 #pragma unroll
                     for (int c = 0; c < 4; ++c)
                         if (16 * c < p.nbp) {
@@ -343,23 +334,31 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
         // U: RROWS x nbp / 8 units of 8 columns, at most one a lane
         const int units = p.nbp >> 3, ur = lane / units, uj = lane % units;
         const bool has_u = ur < RROWS;
+        // where its pieces go in an operand slot: the leading ones fill the first box, the others the next
+        // two, end to end
+        uint32_t u_to[PIECES];
+#pragma unroll
+        for (int piece = 0; piece < PIECES; ++piece) {
+            const int col8 = piece == 0 ? uj : 8 + (piece - 1) * units + uj;
+            u_to[piece] = T * RA_BYTES + (col8 >> 3) * RB_BOX + q8_sw128(r0 + ur, col8 & 7);
+        }
         const long fb = c0 / BLOCK + lane / RROWS;  // whose scale lanes 0 .. RROWS T - 1 fetch
         const bool fetch = lane < RROWS * T && fb * BLOCK < p.cols;
         const float* scales = p.scale + (fetch ? fb * p.lds : 0) + lane % RROWS;
-        float un[8], sn = 0.f;
+        const U* const ubase = static_cast<const U*>(p.u) + (long)ur * p.ldu + 8 * uj;
+        UnitOfU<U> un;
+        float sn = 0.f;
         auto prefetch = [&](int kb) {
             const int t0 = kb * RK + r0;
-            if (has_u) load_u(p, t0 + ur, 8 * uj, un);
+            un.load(ubase + (long)t0 * p.ldu, has_u && t0 + ur < p.rows ? p.nb - 8 * uj : 0, p.u_vec);
             sn = fetch && t0 + lane % RROWS < p.rows ? scales[t0] : 0.f;
         };
         // U and the scales come straight to registers one block ahead, which covers L2's latency but not
         // HBM's: they are called into L2 RAHEAD blocks before that
-        const char* ubase = static_cast<const char*>(p.u);
-        const int usize = p.u_type == OP_F32 ? 4 : 2;
         auto call = [&](int kb) {
             const int t0 = kb * RK + r0;
             if (has_u && t0 + ur < p.rows && 8 * uj < p.nb)
-                asm volatile("prefetch.global.L2 [%0];" ::"l"(ubase + ((long)(t0 + ur) * p.ldu + 8 * uj) * usize));
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(ubase + (long)t0 * p.ldu));
             if (fetch && t0 + lane % RROWS < p.rows) asm volatile("prefetch.global.L2 [%0];" ::"l"(scales + t0));
         };
         for (int kb = kb0; kb < kb0 + RAHEAD && kb < kb1; ++kb) call(kb);
@@ -369,8 +368,7 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
         for (int kb = kb0; kb < kb1; ++kb) {
             float u[8];
             const float sc = sn;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) u[j] = un[j];
+            un.values(u);
             if (kb + 1 < kb1) prefetch(kb + 1);
             if (kb + RAHEAD < kb1) call(kb + RAHEAD);
             bool got = true;
@@ -393,18 +391,18 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
             }
             if (lane == 0) mbar_arrive(raw_empty(s));  // after the shuffles: every lane has read its codes
             if (has_u) {
-                for (int piece = 0; piece < p.pieces; ++piece) {
+                // The next piece of a value is its upper half-word (cut off, not rounded: three pieces hold all
+                // 24 bits and none can overflow); what is left of it is exact.
+#pragma unroll
+                for (int piece = 0; piece < PIECES; ++piece) {
                     uint32_t h[4];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
+                    for (int j = 0; j < 4; ++j)
                         h[j] = __byte_perm(__float_as_uint(u[2 * j]), __float_as_uint(u[2 * j + 1]), 0x7632);
-                        u[2 * j] = left_of(u[2 * j]);
-                        u[2 * j + 1] = left_of(u[2 * j + 1]);
-                    }
-                    // the leading pieces fill the first box, the others the next two, end to end
-                    const int col8 = piece == 0 ? uj : 8 + (piece - 1) * units + uj;
-                    *reinterpret_cast<uint4*>(op + T * RA_BYTES + (col8 >> 3) * RB_BOX + q8_sw128(r0 + ur, col8 & 7)) =
-                        make_uint4(h[0], h[1], h[2], h[3]);
+                    *reinterpret_cast<uint4*>(op + u_to[piece]) = make_uint4(h[0], h[1], h[2], h[3]);
+                    if (piece + 1 < PIECES)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) u[j] -= __uint_as_float(__float_as_uint(u[j]) & 0xffff0000u);
                 }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -455,7 +453,7 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
 
 // How many clusters of `splits` CTAs run at once on the current device: the GPU's processing
 // clusters differ in size, so this is not the SM count over the size.  Asked once per device.
-template <int T, bool E4M3>
+template <int T, bool E4M3, typename U>
 int clusters_at_once(int splits) {
     static std::atomic<int> known[64][RMAX_SPLIT + 1];
     int dev = 0;
@@ -474,7 +472,7 @@ int clusters_at_once(int splits) {
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (cudaOccupancyMaxActiveClusters(&n, rank_kernel<T, E4M3>, &cfg) != cudaSuccess || n < 1) {
+    if (cudaOccupancyMaxActiveClusters(&n, rank_kernel<T, E4M3, U>, &cfg) != cudaSuccess || n < 1) {
         cudaGetLastError();
         return 1;
     }
@@ -482,19 +480,19 @@ int clusters_at_once(int splits) {
     return n;
 }
 
-template <int T, bool E4M3>
+template <int T, bool E4M3, typename U>
 void launch(const RankCkpt8& a, RParams p, cudaStream_t s) {
     typedef RShape<T> S;
     static DeviceOnce once;
     once([] {
-        cudaFuncSetAttribute(rank_kernel<T, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+        cudaFuncSetAttribute(rank_kernel<T, E4M3, U>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
     });
     const long tiles = (a.cols + T * 128 - 1) / (T * 128);
     // slices per tile: the least rounds of clusters times blocks of a slice
     p.splits = 1;
     long best = -1;
     for (int n = 1; n <= RMAX_SPLIT && n <= p.nk; ++n) {
-        const long at_once = clusters_at_once<T, E4M3>(n);
+        const long at_once = clusters_at_once<T, E4M3, U>(n);
         const long cost = (tiles + at_once - 1) / at_once * ((p.nk + n - 1) / n);
         if (best < 0 || cost < best) {
             best = cost;
@@ -515,7 +513,14 @@ void launch(const RankCkpt8& a, RParams p, cudaStream_t s) {
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, rank_kernel<T, E4M3>, maps, p);
+    cudaLaunchKernelEx(&cfg, rank_kernel<T, E4M3, U>, maps, p);
+}
+
+template <int T, bool E4M3>
+void launch(const RankCkpt8& a, const RParams& p, cudaStream_t s) {
+    if (a.u.type == OP_F32) launch<T, E4M3, float>(a, p, s);
+    else if (a.u.type == OP_F16) launch<T, E4M3, f16>(a, p, s);
+    else launch<T, E4M3, __nv_bfloat16>(a, p, s);
 }
 
 }  // namespace
@@ -528,8 +533,8 @@ void rank_ckpt8(const RankCkpt8& a, cudaStream_t s) {
     RParams p;
     p.rows = (int)a.rows; p.nk = (int)((a.rows + RK - 1) / RK); p.nb = a.nb; p.nbp = (a.nb + 15) / 16 * 16;
     p.cols = a.cols;
-    p.u = a.u.p; p.u_type = a.u.type; p.u_vec = vec4(a.u) ? 1 : 0; p.ldu = a.u.ld;
-    p.pieces = a.u.type == OP_F32 ? 3 : a.u.type == OP_F16 ? 2 : 1;
+    p.u = a.u.p; p.ldu = a.u.ld;
+    p.u_vec = a.nb % 8 == 0 && a.u.ld * op_bytes(a.u.type) % 8 == 0 && reinterpret_cast<uintptr_t>(a.u.p) % 8 == 0;
     p.scale = a.x.scale; p.lds = a.x.lds; p.alpha = a.alpha;
     p.c = a.c; p.ldc = a.ldc; p.c_vec = vec4(a.c) && a.ldc % 4 == 0 ? 1 : 0; p.accumulate = a.accumulate ? 1 : 0;
     p.splits = 1; p.status = a.status;
