@@ -19,6 +19,7 @@
 #include <cuda.h>
 
 #include <atomic>
+#include <climits>
 #include <cstring>
 #include <type_traits>
 
@@ -331,34 +332,46 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
         constexpr int RPP = 32 / LPR;      // rows of a pass
         const int cw = warp - 8, r0 = RROWS * cw;  // rows r0 .. r0 + RROWS - 1 of each block
         const int cl = lane % LPR, tile = cl >> 4, box = (cl >> 3) & 1, unit = cl & 7;
-        // U: RROWS x nbp / 8 units of 8 columns, at most one a lane
-        const int units = p.nbp >> 3, ur = lane / units, uj = lane % units;
-        const bool has_u = ur < RROWS;
+        // U: RROWS x nbp / 8 units of 8 columns, up to NU a lane
+        constexpr int NU = (RROWS * 8 + 31) / 32;
+        const int units = p.nbp >> 3;
+        int ur[NU], have[NU];  // a unit's row in the warp's part and its columns that exist (0: no unit)
+        const U* from[NU];
         // where its pieces go in an operand slot: the leading ones fill the first box, the others the next
         // two, end to end
-        uint32_t u_to[PIECES];
+        uint32_t u_to[NU][PIECES];
 #pragma unroll
-        for (int piece = 0; piece < PIECES; ++piece) {
-            const int col8 = piece == 0 ? uj : 8 + (piece - 1) * units + uj;
-            u_to[piece] = T * RA_BYTES + (col8 >> 3) * RB_BOX + q8_sw128(r0 + ur, col8 & 7);
+        for (int i = 0; i < NU; ++i) {
+            const int q = lane + 32 * i, uj = q % units;
+            ur[i] = q / units;
+            have[i] = ur[i] < RROWS ? p.nb - 8 * uj : INT_MIN;
+            from[i] = static_cast<const U*>(p.u) + (long)(r0 + ur[i]) * p.ldu + 8 * uj;
+#pragma unroll
+            for (int piece = 0; piece < PIECES; ++piece) {
+                const int col8 = piece == 0 ? uj : 8 + (piece - 1) * units + uj;
+                u_to[i][piece] = T * RA_BYTES + (col8 >> 3) * RB_BOX + q8_sw128(r0 + ur[i], col8 & 7);
+            }
         }
         const long fb = c0 / BLOCK + lane / RROWS;  // whose scale lanes 0 .. RROWS T - 1 fetch
         const bool fetch = lane < RROWS * T && fb * BLOCK < p.cols;
         const float* scales = p.scale + (fetch ? fb * p.lds : 0) + lane % RROWS;
-        const U* const ubase = static_cast<const U*>(p.u) + (long)ur * p.ldu + 8 * uj;
-        UnitOfU<U> un;
+        UnitOfU<U> un[NU];
         float sn = 0.f;
         auto prefetch = [&](int kb) {
             const int t0 = kb * RK + r0;
-            un.load(ubase + (long)t0 * p.ldu, has_u && t0 + ur < p.rows ? p.nb - 8 * uj : 0, p.u_vec);
+#pragma unroll
+            for (int i = 0; i < NU; ++i)
+                un[i].load(from[i] + (long)kb * RK * p.ldu, t0 + ur[i] < p.rows ? have[i] : 0, p.u_vec);
             sn = fetch && t0 + lane % RROWS < p.rows ? scales[t0] : 0.f;
         };
         // U and the scales come straight to registers one block ahead, which covers L2's latency but not
         // HBM's: they are called into L2 RAHEAD blocks before that
         auto call = [&](int kb) {
             const int t0 = kb * RK + r0;
-            if (has_u && t0 + ur < p.rows && 8 * uj < p.nb)
-                asm volatile("prefetch.global.L2 [%0];" ::"l"(ubase + (long)t0 * p.ldu));
+#pragma unroll
+            for (int i = 0; i < NU; ++i)
+                if (have[i] > 0 && t0 + ur[i] < p.rows)
+                    asm volatile("prefetch.global.L2 [%0];" ::"l"(from[i] + (long)kb * RK * p.ldu));
             if (fetch && t0 + lane % RROWS < p.rows) asm volatile("prefetch.global.L2 [%0];" ::"l"(scales + t0));
         };
         for (int kb = kb0; kb < kb0 + RAHEAD && kb < kb1; ++kb) call(kb);
@@ -366,9 +379,10 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
         int s = 0, o = 0;
         uint32_t ph = 0, oph = 0;
         for (int kb = kb0; kb < kb1; ++kb) {
-            float u[8];
+            float u[NU][8];
             const float sc = sn;
-            un.values(u);
+#pragma unroll
+            for (int i = 0; i < NU; ++i) un[i].values(u[i]);
             if (kb + 1 < kb1) prefetch(kb + 1);
             if (kb + RAHEAD < kb1) call(kb + RAHEAD);
             bool got = true;
@@ -390,19 +404,21 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
                     codes_to_bf16<E4M3>(w[i], sr);
             }
             if (lane == 0) mbar_arrive(raw_empty(s));  // after the shuffles: every lane has read its codes
-            if (has_u) {
-                // The next piece of a value is its upper half-word (cut off, not rounded: three pieces hold all
-                // 24 bits and none can overflow); what is left of it is exact.
+            // The next piece of a value is its upper half-word (cut off, not rounded: three pieces hold all
+            // 24 bits and none can overflow); what is left of it is exact.
+#pragma unroll
+            for (int i = 0; i < NU; ++i) {
+                if (have[i] == INT_MIN) break;
 #pragma unroll
                 for (int piece = 0; piece < PIECES; ++piece) {
                     uint32_t h[4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
-                        h[j] = __byte_perm(__float_as_uint(u[2 * j]), __float_as_uint(u[2 * j + 1]), 0x7632);
-                    *reinterpret_cast<uint4*>(op + u_to[piece]) = make_uint4(h[0], h[1], h[2], h[3]);
+                        h[j] = __byte_perm(__float_as_uint(u[i][2 * j]), __float_as_uint(u[i][2 * j + 1]), 0x7632);
+                    *reinterpret_cast<uint4*>(op + u_to[i][piece]) = make_uint4(h[0], h[1], h[2], h[3]);
                     if (piece + 1 < PIECES)
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) u[j] -= __uint_as_float(__float_as_uint(u[j]) & 0xffff0000u);
+                        for (int j = 0; j < 8; ++j) u[i][j] -= __uint_as_float(__float_as_uint(u[i][j]) & 0xffff0000u);
                 }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
