@@ -175,13 +175,12 @@ __device__ __forceinline__ void unpairs(const uint64_t v[2], float o[4]) {
 
 // ---------------------------------------------------------------------------------------
 // Block scale.  top = m 2^k (1 <= m < 2) and amax = a 2^j: the smallest power of two s with
-// amax <= top s is 2^(j - k), or 2^(j - k + 1) where a > m: one comparison of mantissa bits.
-// 448 = 1.75 * 2^8, 127 = 1.984375 * 2^6.  s >= 2^-126 keeps s and 1 / s normal, which is what
-// an all-zero block (and a subnormal amax) gets.
+// amax <= top s is 2^(j - k), or 2^(j - k + 1) where a > m: adding the mantissa's distance from m
+// to its end carries into the exponent just then.  448 = 1.75 * 2^8, 127 = 1.984375 * 2^6.
+// s >= 2^-126 keeps s and 1 / s normal, which is what an all-zero block (and a subnormal amax) gets.
 __device__ __forceinline__ uint32_t scale_bits(uint32_t amax_bits, bool e4m3) {
-    const uint32_t k = e4m3 ? 8u : 6u, m = e4m3 ? 0x600000u : 0x7e0000u;
-    const uint32_t e = (amax_bits >> 23) + ((amax_bits & 0x7fffffu) > m ? 1u : 0u);
-    return max(e, k + 1) - k << 23;
+    const uint32_t k = e4m3 ? 8u : 6u, room = e4m3 ? 0x1fffffu : 0x1ffffu;
+    return max((amax_bits + room) & 0x7f800000u, (k + 1) << 23) - (k << 23);
 }
 // 1 / s of a power of two: exponent 254 - e
 __device__ __forceinline__ float inverse_pow2(uint32_t s_bits) { return __uint_as_float((254u << 23) - s_bits); }
@@ -315,10 +314,14 @@ __device__ __forceinline__ float rcp(float v) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
 }
-// Q and exp(-z^2 / 2) of a = min(|z|, 16): beyond 16 both are 0
+// a = -min(|z|, 16): beyond 16 Q and exp(-z^2 / 2) are 0
+__device__ __forceinline__ uint64_t minus_abs(float z0, float z1) {
+    return pair(fmaxf(-fabsf(z0), -16.f), fmaxf(-fabsf(z1), -16.f));
+}
+// Q and exp(-z^2 / 2)
 __device__ __forceinline__ void normal_tail(uint64_t a, uint64_t& q, uint64_t& e) {
     const float2 x = unpair(mul2(mul2(a, a), pair(-0.72134752044448170f)));  // -z^2 / 2 in powers of two
-    const float2 d = unpair(fma2(a, pair(0.3f), pair(1.0f)));
+    const float2 d = unpair(fma2(a, pair(-0.3f), pair(1.0f)));
     const uint64_t t = pair(rcp(d.x), rcp(d.y));
     e = pair(ex2(x.x), ex2(x.y));
     uint64_t r = pair(0.03840748965740204f);
@@ -334,17 +337,16 @@ __device__ __forceinline__ void normal_tail(uint64_t a, uint64_t& q, uint64_t& e
 }
 // z Phi(z) = max(z, 0) - |z| Q
 __device__ __forceinline__ uint64_t gelu2(float z0, float z1) {
-    const uint64_t a = pair(fminf(fabsf(z0), 16.f), fminf(fabsf(z1), 16.f));
+    const uint64_t a = minus_abs(z0, z1);
     uint64_t q, e;
     normal_tail(a, q, e);
-    return fma2(mul2(a, pair(-1.0f)), q, pair(max_nan(z0, 0.f), max_nan(z1, 0.f)));
+    return fma2(a, q, pair(max_nan(z0, 0.f), max_nan(z1, 0.f)));
 }
 // Phi(z) + z phi(z), Phi(z) = [z > 0] - sign(z) Q
 __device__ __forceinline__ uint64_t gelu_grad2(uint64_t z) {
     const float2 f = unpair(z);
-    const uint64_t a = pair(fminf(fabsf(f.x), 16.f), fminf(fabsf(f.y), 16.f));
     uint64_t q, e;
-    normal_tail(a, q, e);
+    normal_tail(minus_abs(f.x, f.y), q, e);
     const float2 u = unpair(q);
     const uint64_t sq = pair(f.x > 0.f ? -u.x : u.x, f.y > 0.f ? -u.y : u.y);
     const uint64_t step = pair(f.x > 0.f ? 1.f : 0.f, f.y > 0.f ? 1.f : 0.f);

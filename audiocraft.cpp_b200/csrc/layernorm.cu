@@ -18,24 +18,37 @@ namespace {
 using namespace c8;
 
 // ---------------------------------------------------------------------------------------
-// sums of N values over the W warps of a row; slot: W * N floats of shared memory that nobody
-// else uses between two calls (the caller alternates between two)
-template <int W, int N>
-__device__ __forceinline__ void row_sum(float* v, float* slot, int wid, int lane, int bar) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = warp_sum(v[i]);
-    if (W == 1) return;
-    if (lane == 0)
-#pragma unroll
-        for (int i = 0; i < N; ++i) slot[wid * N + i] = v[i];
+// The sum of one value, and of two, over the W warps of a row.  slot: W (2 W) floats of shared memory
+// that nobody else uses between two calls (the caller alternates between two); bar: the row's
+// own named barrier.
+template <int W>
+__device__ __forceinline__ float row_sum(float v, float* slot, int wid, int lane, int bar) {
+    v = warp_sum(v);
+    if (W == 1) return v;
+    if (lane == 0) slot[wid] = v;
     asm volatile("bar.sync %0, %1;" ::"r"(bar), "n"(W * 32) : "memory");
+    float s = 0.f;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        float s = 0.f;
+    for (int w = 0; w < W; ++w) s += slot[w];
+    return s;
+}
+template <int W>
+__device__ __forceinline__ float2 row_sum2(float a, float b, float2* slot, int wid, int lane, int bar) {
+    // after the first exchange the lower half-warp holds a's pairs and the upper one b's
+    const bool up = lane & 16;
+    float v = (up ? b : a) + __shfl_xor_sync(FULL_WARP, up ? a : b, 16);
 #pragma unroll
-        for (int w = 0; w < W; ++w) s += slot[w * N + i];
-        v[i] = s;
+    for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(FULL_WARP, v, o);
+    if (W == 1) return make_float2(__shfl_sync(FULL_WARP, v, 0), __shfl_sync(FULL_WARP, v, 16));
+    if ((lane & 15) == 0) reinterpret_cast<float*>(slot + wid)[lane >> 4] = v;
+    asm volatile("bar.sync %0, %1;" ::"r"(bar), "n"(W * 32) : "memory");
+    float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+        s.x += slot[w].x;
+        s.y += slot[w].y;
     }
+    return s;
 }
 
 struct FwdParams {
@@ -85,9 +98,8 @@ __global__ void __launch_bounds__(W * G * 32) ln_fwd_kernel(const FwdParams p) {
             sum2 = add2(sum2, add2(v[k][0], v[k][1]));
         }
         if (row + step < p.rows) fetch();
-        float sum = unpair(sum2).x + unpair(sum2).y;
-        row_sum<W, 1>(&sum, slots[0][grp], wid, lane, 1 + grp);
-        const float mean = sum * p.inv_dim;
+        const float mean =
+            row_sum<W>(unpair(sum2).x + unpair(sum2).y, slots[0][grp], wid, lane, 1 + grp) * p.inv_dim;
         const uint64_t minus = pair(-mean);
         uint64_t sq2 = 0;
 #pragma unroll
@@ -102,8 +114,7 @@ __global__ void __launch_bounds__(W * G * 32) ln_fwd_kernel(const FwdParams p) {
             }
             sq2 = fma2(d[0], d[0], fma2(d[1], d[1], sq2));
         }
-        float sq = unpair(sq2).x + unpair(sq2).y;
-        row_sum<W, 1>(&sq, slots[1][grp], wid, lane, 1 + grp);
+        const float sq = row_sum<W>(unpair(sq2).x + unpair(sq2).y, slots[1][grp], wid, lane, 1 + grp);
         const float rstd = rsqrtf(sq * p.inv_dim + p.eps);
         if (wid == 0 && lane == 0) {
             p.mean[row] = mean;
@@ -173,14 +184,14 @@ __global__ void __launch_bounds__(W * G * 32) ln_fwd_kernel(const FwdParams p) {
 // their use (cp.async: nobody else reads them, so no barrier is needed), which keeps enough
 // bytes in flight at one CTA of 16 warps an SM, all that the sums' registers leave room for.
 constexpr int BWD_WARPS = 16;
-constexpr int BWD_NCH = 4;
+constexpr int BWD_NCH = 4;  // blocks of 128 columns a warp holds at most
 constexpr int BWD_DEPTH = 4;
 
 struct BwdParams {
     long rows, ldy, ldx, lddx;  // strides in bytes
     const char *dy, *x, *add;
     char* dx;
-    int dy_half, x_half, x_e4m3, dx_wide, dx_half, dim;
+    int dy_half, x_half, dx_wide, dx_half, dim;
     const float *w, *mean, *rstd, *scale;
     long lds;
     float inv_dim;
@@ -200,16 +211,16 @@ __device__ __forceinline__ void read4(const unsigned char* p, bool half, float v
     else unpack4(*reinterpret_cast<const uint2*>(p), v, __nv_bfloat16());
 }
 
-// DB, XB: bytes of an element of dy and of the kept input (1: codes); AHEAD: lanes copy ahead and
-// everything moves four elements at a time.  Columns past the row's end read as x = 0 and dy = 0,
+// DB, XB: bytes of an element of dy and of the kept input (1: codes, E4M3 or I8); AHEAD: lanes copy
+// ahead, everything moves four elements at a time and w stays in registers.  Columns past the row's end read as x = 0 and dy = 0,
 // so that they add nothing to any sum whatever their h is.
-template <int DB, int XB, int W, bool AHEAD>
+template <int DB, int XB, bool E4M3, int W, int NCH, bool AHEAD>
 __global__ void __launch_bounds__(BWD_WARPS * 32) ln_bwd_kernel(const BwdParams p) {
-    constexpr int G = BWD_WARPS / W, NCH = BWD_NCH, THREADS = BWD_WARPS * 32, NEXT = W * BLOCK;
+    constexpr int G = BWD_WARPS / W, THREADS = BWD_WARPS * 32, NEXT = W * BLOCK;
     // a stage: per block a lane's four of dy and four of x
     constexpr int X_OFF = NCH * 4 * DB * THREADS, STAGE = X_OFF + NCH * 4 * XB * THREADS;
     constexpr int DEPTH = STAGE * BWD_DEPTH <= 160 * 1024 ? BWD_DEPTH : 2;
-    __shared__ float slots[2][G][W * 2];
+    __shared__ float2 slots[2][G][W];
     extern __shared__ __align__(16) unsigned char room[];  // the stages; at the end [2][dim] sums
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, grp = warp / W, wid = warp % W, t = threadIdx.x;
     const int first_c = wid * BLOCK + first_col<AHEAD>(lane), left = p.dim - first_c;
@@ -218,14 +229,27 @@ __global__ void __launch_bounds__(BWD_WARPS * 32) ln_bwd_kernel(const BwdParams 
     const char *dy = p.dy + first * p.ldy + first_c * DB, *x = p.x + first * p.ldx + first_c * XB;
     // lane k fetches block k's scale of the next row; every lane its mean and rstd
     const bool scales = XB == 1 && lane < NCH && (lane * W + wid) * BLOCK < p.dim;
-    const float* scale_at = p.scale + (scales ? (long)(lane * W + wid) * p.lds : 0);
+    const float *scale_at = p.scale + (scales ? (long)(lane * W + wid) * p.lds : 0) + first, *mean_at = p.mean + first,
+                *rstd_at = p.rstd + first;
     float next_scale = 0.f, next_mean = 0.f, next_rstd = 0.f;
-    auto fetch = [&](long row) {
-        if (row >= p.rows) return;
-        if (scales) next_scale = scale_at[row];
-        next_mean = p.mean[row];
-        next_rstd = p.rstd[row];
+    auto fetch = [&](bool any) {
+        if (any) {
+            if (scales) next_scale = *scale_at;
+            next_mean = *mean_at;
+            next_rstd = *rstd_at;
+        }
+        scale_at += step;
+        mean_at += step;
+        rstd_at += step;
     };
+    uint64_t w2[AHEAD ? NCH : 1][2];
+    if (AHEAD)
+#pragma unroll
+        for (int k = 0; k < NCH; ++k) {
+            float f[4] = {1.f, 1.f, 1.f, 1.f};
+            if (p.w) load4_const<true>(p.w + first_c + k * NEXT, left - k * NEXT, f);
+            pairs(f, w2[k]);
+        }
     const uint32_t ring = smem_u32(room) + t * 4 * DB, xring = smem_u32(room) + X_OFF + t * 4 * XB;
     long coming = first;
     int slot = 0;
@@ -247,7 +271,7 @@ __global__ void __launch_bounds__(BWD_WARPS * 32) ln_bwd_kernel(const BwdParams 
     if (AHEAD)
 #pragma unroll
         for (int s = 0; s < DEPTH - 1; ++s) ahead();
-    fetch(first);
+    fetch(first < p.rows);
     char* dx = p.dx + first * p.lddx + first_c * (p.dx_wide ? 4 : 2);
     const char* add = p.add + first * p.lddx + first_c * (p.dx_wide ? 4 : 2);
     int stage = 0, turn = 0;
@@ -255,7 +279,7 @@ __global__ void __launch_bounds__(BWD_WARPS * 32) ln_bwd_kernel(const BwdParams 
         uint64_t h[NCH][2], g[NCH][2], red0 = 0, red1 = 0;
         const unsigned char *at = room + stage * STAGE + t * 4 * DB, *xat = room + stage * STAGE + X_OFF + t * 4 * XB;
         const float scale = next_scale, mean = next_mean, rstd = next_rstd;
-        fetch(row + step);
+        fetch(row + step < p.rows);
         if (AHEAD) {
             ahead();
             cp_async_wait<DEPTH - 1>();
@@ -270,12 +294,12 @@ __global__ void __launch_bounds__(BWD_WARPS * 32) ln_bwd_kernel(const BwdParams 
             if (AHEAD) {
                 if (n > 0) {
                     read4<DB>(at + k * THREADS * 4 * DB, p.dy_half, f);
-                    if (XB == 1) decode4(*reinterpret_cast<const uint32_t*>(xat + k * THREADS * 4), p.x_e4m3, q);
+                    if (XB == 1) decode4(*reinterpret_cast<const uint32_t*>(xat + k * THREADS * 4), E4M3, q);
                     else read4<XB == 1 ? 2 : XB>(xat + k * THREADS * 4 * XB, p.x_half, q);
                 }
             } else {
                 load4_bytes<DB, false>(dy + k * NEXT * DB, p.dy_half, n, f);
-                if (XB == 1) decode4(load_codes<false>(reinterpret_cast<const uint8_t*>(x) + k * NEXT, n), p.x_e4m3, q);
+                if (XB == 1) decode4(load_codes<false>(reinterpret_cast<const uint8_t*>(x) + k * NEXT, n), E4M3, q);
                 else load4_bytes<XB == 1 ? 2 : XB, false>(x + k * NEXT * XB, p.x_half, n, q);
             }
             uint64_t d2[2], x2[2];
@@ -290,12 +314,14 @@ __global__ void __launch_bounds__(BWD_WARPS * 32) ln_bwd_kernel(const BwdParams 
                 db[k][i] = add2(db[k][i], d2[i]);
                 g[k][i] = d2[i];
             }
-            if (p.w) {
-                uint64_t w2[2];
-                load4_const<AHEAD>(p.w + first_c + k * NEXT, n, f);
-                pairs(f, w2);
-                g[k][0] = mul2(g[k][0], w2[0]);
-                g[k][1] = mul2(g[k][1], w2[1]);
+            if (AHEAD) {
+                g[k][0] = mul2(g[k][0], w2[k][0]);
+                g[k][1] = mul2(g[k][1], w2[k][1]);
+            } else if (p.w) {
+                load4_const<false>(p.w + first_c + k * NEXT, n, f);
+                pairs(f, w2[0]);
+                g[k][0] = mul2(g[k][0], w2[0][0]);
+                g[k][1] = mul2(g[k][1], w2[0][1]);
             }
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -307,10 +333,10 @@ __global__ void __launch_bounds__(BWD_WARPS * 32) ln_bwd_kernel(const BwdParams 
             dy += step * p.ldy;
             x += step * p.ldx;
         }
-        float red[2] = {unpair(red0).x + unpair(red0).y, unpair(red1).x + unpair(red1).y};
-        row_sum<W, 2>(red, slots[turn][grp], wid, lane, 1 + grp);
+        const float2 red = row_sum2<W>(unpair(red0).x + unpair(red0).y, unpair(red1).x + unpair(red1).y,
+                                       slots[turn][grp], wid, lane, 1 + grp);
         turn ^= 1;
-        const uint64_t c1 = pair(-red[0] * p.inv_dim), c2 = pair(-red[1] * p.inv_dim);
+        const uint64_t c1 = pair(-red.x * p.inv_dim), c2 = pair(-red.y * p.inv_dim);
 #pragma unroll
         for (int k = 0; k < NCH; ++k) {
             if ((k * W + wid) * BLOCK >= p.dim) break;
@@ -358,9 +384,9 @@ __global__ void __launch_bounds__(BWD_WARPS * 32) ln_bwd_kernel(const BwdParams 
     for (int c = threadIdx.x; c < 2 * p.dim; c += THREADS) out[c] = sums[c];
 }
 
-template <int DB, int XB>
+template <int DB, int XB, int NCH>
 constexpr int bwd_room() {
-    constexpr int stage = BWD_WARPS * 32 * BWD_NCH * 4 * (DB + XB);
+    constexpr int stage = BWD_WARPS * 32 * NCH * 4 * (DB + XB);
     return stage * BWD_DEPTH <= 160 * 1024 ? stage * BWD_DEPTH : 2 * stage;
 }
 
@@ -435,32 +461,43 @@ void fwd_by_dim(const FwdParams& p, bool vec, cudaStream_t s) {
     else launch_fwd<T, 8, 8, 1>(p, vec, s);
 }
 
-template <int DB, int XB, int W, bool AHEAD>
+template <int DB, int XB, bool E4M3, int W, int NCH, bool AHEAD>
 void launch_bwd(const BwdParams& p, int ctas, cudaStream_t s) {
-    constexpr int most = 2 * BWD_NCH * BLOCK * W * (int)sizeof(float);  // sums of the widest row
-    constexpr int smem = AHEAD && bwd_room<DB, XB>() > most ? bwd_room<DB, XB>() : most;
+    constexpr int most = 2 * NCH * BLOCK * W * (int)sizeof(float);  // sums of the widest row
+    constexpr int smem = AHEAD && bwd_room<DB, XB, NCH>() > most ? bwd_room<DB, XB, NCH>() : most;
     static DeviceOnce once;
     once([] {
-        cudaFuncSetAttribute(ln_bwd_kernel<DB, XB, W, AHEAD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        cudaFuncSetAttribute(ln_bwd_kernel<DB, XB, E4M3, W, NCH, AHEAD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             smem);
     });
-    ln_bwd_kernel<DB, XB, W, AHEAD><<<ctas, BWD_WARPS * 32, smem, s>>>(p);
+    ln_bwd_kernel<DB, XB, E4M3, W, NCH, AHEAD><<<ctas, BWD_WARPS * 32, smem, s>>>(p);
 }
 
-template <int DB, int XB, int W>
+// three blocks a warp where they are enough (1536 columns on four warps): fewer registers, no idle block
+template <int DB, int XB, bool E4M3, int W>
 void launch_bwd(const BwdParams& p, bool vec, int ctas, cudaStream_t s) {
-    if (vec) launch_bwd<DB, XB, W, true>(p, ctas, s);
-    else launch_bwd<DB, XB, W, false>(p, ctas, s);
+    if (!vec) launch_bwd<DB, XB, E4M3, W, BWD_NCH, false>(p, ctas, s);
+    else if (p.dim <= 3 * W * BLOCK) launch_bwd<DB, XB, E4M3, W, 3, true>(p, ctas, s);
+    else launch_bwd<DB, XB, E4M3, W, BWD_NCH, true>(p, ctas, s);
 }
 
-template <int DB, int XB>
+template <int DB, int XB, bool E4M3>
 void bwd_by_dim(const BwdParams& p, bool vec, int ctas, cudaStream_t s) {
     switch (bwd_warps(p.dim)) {
-        case 1: return launch_bwd<DB, XB, 1>(p, vec, ctas, s);
-        case 2: return launch_bwd<DB, XB, 2>(p, vec, ctas, s);
-        case 4: return launch_bwd<DB, XB, 4>(p, vec, ctas, s);
-        case 8: return launch_bwd<DB, XB, 8>(p, vec, ctas, s);
-        default: return launch_bwd<DB, XB, 16>(p, vec, ctas, s);
+        case 1: return launch_bwd<DB, XB, E4M3, 1>(p, vec, ctas, s);
+        case 2: return launch_bwd<DB, XB, E4M3, 2>(p, vec, ctas, s);
+        case 4: return launch_bwd<DB, XB, E4M3, 4>(p, vec, ctas, s);
+        case 8: return launch_bwd<DB, XB, E4M3, 8>(p, vec, ctas, s);
+        default: return launch_bwd<DB, XB, E4M3, 16>(p, vec, ctas, s);
     }
+}
+
+template <int DB>
+void bwd_by_type(const BwdParams& p, int xb, bool e4m3, bool vec, int ctas, cudaStream_t s) {
+    if (xb == 4) bwd_by_dim<DB, 4, false>(p, vec, ctas, s);
+    else if (xb == 2) bwd_by_dim<DB, 2, false>(p, vec, ctas, s);
+    else if (e4m3) bwd_by_dim<DB, 1, true>(p, vec, ctas, s);
+    else bwd_by_dim<DB, 1, false>(p, vec, ctas, s);
 }
 
 }  // namespace
@@ -488,7 +525,7 @@ void layernorm_train_bwd(const LnBwd& a, cudaStream_t s) {
     p.dy = static_cast<const char*>(a.dy.p); p.dy_half = a.dy.type == OP_F16;
     p.x = a.x8.q ? reinterpret_cast<const char*>(a.x8.q) : static_cast<const char*>(a.x.p);
     p.ldx = a.x8.q ? a.x8.ldq : a.x.ld * op_bytes(a.x.type);
-    p.x_half = a.x.type == OP_F16; p.x_e4m3 = a.x8.e4m3; p.scale = a.x8.scale; p.lds = a.x8.lds;
+    p.x_half = a.x.type == OP_F16; p.scale = a.x8.scale; p.lds = a.x8.lds;
     p.add = static_cast<const char*>(a.add.p); p.dx = static_cast<char*>(const_cast<void*>(a.dx.p));
     p.dx_wide = a.dx.type == OP_F32; p.dx_half = a.dx.type == OP_F16; p.dim = a.dim;
     p.w = a.w; p.mean = a.mean; p.rstd = a.rstd; p.inv_dim = 1.0f / (float)a.dim; p.part = a.space;
@@ -496,15 +533,8 @@ void layernorm_train_bwd(const LnBwd& a, cudaStream_t s) {
     const int ctas = a.rows > 0 ? bwd_ctas(a.rows, a.dim) : 0;
     if (ctas) {
         const int xb = a.x8.q ? 1 : op_bytes(a.x.type);
-        if (op_bytes(a.dy.type) == 4) {
-            if (xb == 1) bwd_by_dim<4, 1>(p, vec, ctas, s);
-            else if (xb == 2) bwd_by_dim<4, 2>(p, vec, ctas, s);
-            else bwd_by_dim<4, 4>(p, vec, ctas, s);
-        } else {
-            if (xb == 1) bwd_by_dim<2, 1>(p, vec, ctas, s);
-            else if (xb == 2) bwd_by_dim<2, 2>(p, vec, ctas, s);
-            else bwd_by_dim<2, 4>(p, vec, ctas, s);
-        }
+        if (op_bytes(a.dy.type) == 4) bwd_by_type<4>(p, xb, a.x8.e4m3, vec, ctas, s);
+        else bwd_by_type<2>(p, xb, a.x8.e4m3, vec, ctas, s);
     }
     if (a.dw || a.db)
         launch_pdl(ln_sums_kernel, dim3((2 * a.dim + 31) / 32), dim3(1024), 0, s, (const float*)a.space, ctas, a.dim,
