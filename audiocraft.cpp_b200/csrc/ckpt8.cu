@@ -114,7 +114,9 @@ __global__ void __launch_bounds__(THREADS) store_kernel(const T* x, long ldx, lo
         });
 }
 
-// one CTA per 128 x 128 block: a first pass for the maximum, a second that finds the block in L1
+// One CTA per 128 x 128 block, which its threads hold in registers between finding the largest value
+// and writing the codes: every element is read once.
+constexpr int SQUARE_ROWS = BLOCK / (THREADS / 32);  // rows of a warp
 template <typename T, bool VEC, bool E4M3>
 __global__ void __launch_bounds__(THREADS) store_square_kernel(const T* x, long ldx, long rows, long cols, Q8 out) {
     __shared__ uint32_t top[THREADS / 32];
@@ -122,27 +124,46 @@ __global__ void __launch_bounds__(THREADS) store_square_kernel(const T* x, long 
     const long c0 = (long)blockIdx.x * BLOCK + first_col<VEC>(lane);
     const int n = cols - c0 < BLOCK ? (int)(cols - c0) : BLOCK;
     for (long rb = blockIdx.y; rb * BLOCK < rows; rb += gridDim.y) {
-        const long r0 = rb * BLOCK, r1 = r0 + BLOCK < rows ? r0 + BLOCK : rows;
+        const long r0 = rb * BLOCK + warp * SQUARE_ROWS;
+        const int nr = rows - r0 < SQUARE_ROWS ? (int)(rows - r0) : SQUARE_ROWS;
+        Raw4<T, VEC> held[SQUARE_ROWS];
+        const T* at = x + r0 * ldx + c0;
+#pragma unroll
+        for (int r = 0; r < SQUARE_ROWS; ++r) held[r].load(at + r * ldx, r < nr ? n : 0);
         uint32_t m = 0, any = 0;
-        for (long r = r0 + warp; r < r1; r += THREADS / 32) {
+#pragma unroll
+        for (int r = 0; r < SQUARE_ROWS; ++r) {
             float v[4];
-            load4<T, VEC>(x + r * ldx + c0, n, v);
-            m = max(m, largest_finite(v));
+            held[r].values(v);
             any = max(any, largest(v));
         }
         const bool bad = __syncthreads_or(any >= 0x7f800000u);
+        if (bad) {
+#pragma unroll
+            for (int r = 0; r < SQUARE_ROWS; ++r) {
+                float v[4];
+                held[r].values(v);
+                m = max(m, largest_finite(v));
+            }
+        } else {
+            m = any;
+        }
         m = __reduce_max_sync(FULL_WARP, m);
         if (lane == 0) top[warp] = m;
         __syncthreads();
 #pragma unroll
         for (int w = 0; w < THREADS / 32; ++w) m = max(m, top[w]);
         const uint32_t s = scale_bits(m, E4M3);
-        for (long r = r0 + warp; r < r1; r += THREADS / 32) {
+        const float inv = inverse_pow2(s);
+        uint8_t* q = out.q + r0 * out.ldq + c0;
+#pragma unroll
+        for (int r = 0; r < SQUARE_ROWS; ++r) {
             float v[4];
-            load4<T, VEC>(x + r * ldx + c0, n, v);
-            store_codes<VEC>(out.q + r * out.ldq + c0, n, encode4(v, inverse_pow2(s), E4M3, bad));
+            held[r].values(v);
+            store_codes<VEC>(q + r * out.ldq, r < nr ? n : 0, encode4(v, inv, E4M3, bad));
         }
         if (threadIdx.x == 0) out.scale[(long)blockIdx.x * out.lds + rb] = __uint_as_float(s);
+        __syncthreads();  // top is read before the next block's is written
     }
 }
 
