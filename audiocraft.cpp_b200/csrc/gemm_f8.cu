@@ -260,9 +260,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) gemm_f8_kernel(const __grid_const
                 // W's scales: [k-block][n-block], or [n-block][k-block] of a weight stored [K][N]
                 const float* sw = p.sw + (w ? (MN ? n / 128 * p.ldsw : n / 128) : 0);
                 for (int kb = 0; kb < p.nk; ++kb) {
-                    bool got = true;
-                    if (lane == 0) got = mbar_wait_inline(empty_bar(s), ph ^ 1, p.status, 35);
-                    if (!__shfl_sync(FULL_WARP, got ? 1 : 0, 0)) { ok = false; break; }
+                    if (!__all_sync(FULL_WARP, mbar_wait_inline(empty_bar(s), ph ^ 1, p.status, 35))) { ok = false; break; }
                     const uint32_t to = ring + slot * SCALE_LD * 4;
                     if (whole) {
                         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + 16 * lane), "l"(sx) : "memory");
@@ -333,9 +331,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) gemm_f8_kernel(const __grid_const
 #pragma unroll
             for (int i = 0; i < S::HALF / 2; ++i) acc[i] = 0;
             for (int kb = 0; kb < p.nk; ++kb) {
-                bool got = true;
-                if (lane == 0) got = mbar_wait_inline(tfull(b), bph, p.status, 34);
-                if (!__shfl_sync(FULL_WARP, got ? 1 : 0, 0)) { ok = false; break; }
+                // every lane waits (a lane that waited for its warp would cost the warp a detour); they agree
+                if (!__all_sync(FULL_WARP, mbar_wait_inline(tfull(b), bph, p.status, 34))) { ok = false; break; }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const float* at = scales + slot * SCALE_LD;
                 const uint64_t sc = pair(at[quad * 32 + lane] * at[BM + (BN == 256 ? half : 0)]);

@@ -9,11 +9,10 @@
 //              128-byte-swizzled MN-major layout; the block's rows of U, cut into bf16 pieces that add
 //              up to it exactly (one for bf16, two for f16, three for fp32): both operands of the
 //              MMA have to be bf16, and the product keeps all of U
-//   warp 1     tcgen05 MMAs: one accumulator for the leading pieces, one for the others
+//   warp 1     tcgen05 MMAs, the pieces side by side as their columns (one reading of the X tile feeds all)
 //   warps 4-7  the sums: the tensor cores cut each addition into the accumulator off below its last bit
 //              (measured: a relative 2^-24 downwards per 16 rows, 5e-6 over 4000 rows), so the
-//              leading accumulator is emptied into fp32 registers every 256 rows, two of them in turn;
-//              the others are at least 2^-8 smaller and are added once, at the end
+//              accumulators are emptied into fp32 registers every 256 rows (two in turn where they fit)
 // The slices of a column tile form a cluster and add their sums in order through distributed
 // shared memory: no atomics, the same bits every time.
 #include <cuda.h>
@@ -34,7 +33,7 @@ using namespace c8;
 using namespace tc;
 
 constexpr int RK = 64;                   // rows t of a block
-constexpr int RGROUP = 4;                // blocks between two emptyings of the leading accumulator
+constexpr int RGROUP = 4;                // blocks between two emptyings of the accumulators
 constexpr int RCONV = 16;                // converting warps
 constexpr int RAHEAD = 8;
 constexpr int RROWS = RK / RCONV;        // rows of a block each takes
@@ -43,19 +42,20 @@ constexpr int RA_BYTES = 128 * RK * 2;   // bf16 operand of 128 columns
 constexpr int RB_BOX = RK * 64 * 2;      // 64 columns of pieces
 constexpr int RMAX_SPLIT = 8;            // portable cluster size
 
-// T: tiles of 128 columns per CTA
-template <int T>
+// T: tiles of 128 columns per CTA; P: pieces of U
+template <int T, int P>
 struct RShape {
     static constexpr int RAW = T * 128 * RK;
     static constexpr int RAWS = T == 2 ? 6 : 8;
-    static constexpr int OP = T * RA_BYTES + 3 * RB_BOX;
+    static constexpr int OP = T * RA_BYTES + P * RB_BOX;
     static constexpr int OPS = T == 2 ? 2 : 3;
+    static constexpr int ACC = P * 64;                      // TMEM columns of a tile's accumulator
+    static constexpr int BUFS = 2 * T * ACC <= 512 ? 2 : 1;  // of all tiles' accumulators
+    static constexpr int TMEM = BUFS * T * ACC <= 128 ? 128 : BUFS * T * ACC <= 256 ? 256 : 512;
     static constexpr int RAW_OFF = OPS * OP;
     static constexpr int BAR_OFF = RAW_OFF + RAWS * RAW;
-    static constexpr int NBARS = 2 * RAWS + 2 * OPS + 6;
+    static constexpr int NBARS = 2 * RAWS + 2 * OPS + 5;
     static constexpr int SMEM = BAR_OFF + 8 * NBARS + 16 + 1024 /*align*/;
-    static constexpr int TMEM = 256 * T;     // leading: 2 x T x 64 columns, others: T x 128
-    static constexpr int OTHER = 128 * T;    // first column of the others
     static constexpr int LD = T * 128 + 4;   // floats of a row of the sums in shared memory
     static_assert(64 * LD * 4 <= RAW_OFF, "the sums take the operand ring's place");
 };
@@ -148,11 +148,16 @@ struct UnitOfU {
     }
 };
 
-// U: type of U; PIECES bf16 pieces hold all of it
+// bf16 pieces that hold all of a value of U
+template <typename U>
+struct Pieces {
+    static constexpr int N = sizeof(U) == 4 ? 3 : std::is_same<U, f16>::value ? 2 : 1;
+};
+
 template <int T, bool E4M3, typename U>
 __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant__ RMaps maps, const RParams p) {
-    typedef RShape<T> S;
-    constexpr int PIECES = sizeof(U) == 4 ? 3 : std::is_same<U, f16>::value ? 2 : 1;
+    constexpr int PIECES = Pieces<U>::N;
+    typedef RShape<T, PIECES> S;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t base = (raw + 1023) & ~1023u;
@@ -162,10 +167,9 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
     auto raw_empty = [&](int s) { return bars + 8 * (S::RAWS + s); };
     auto op_full = [&](int s) { return bars + 8 * (2 * S::RAWS + s); };
     auto op_empty = [&](int s) { return bars + 8 * (2 * S::RAWS + S::OPS + s); };
-    auto lead_full = [&](int b) { return bars + 8 * (2 * S::RAWS + 2 * S::OPS + b); };
-    auto lead_empty = [&](int b) { return bars + 8 * (2 * S::RAWS + 2 * S::OPS + 2 + b); };
-    const uint32_t all_done = bars + 8 * (2 * S::RAWS + 2 * S::OPS + 4);
-    const uint32_t drained = all_done + 8;
+    auto acc_full = [&](int b) { return bars + 8 * (2 * S::RAWS + 2 * S::OPS + b); };
+    auto acc_empty = [&](int b) { return bars + 8 * (2 * S::RAWS + 2 * S::OPS + 2 + b); };
+    const uint32_t drained = bars + 8 * (2 * S::RAWS + 2 * S::OPS + 4);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::BAR_OFF + 8 * S::NBARS);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const long c0 = (long)blockIdx.x * (T * 128);
@@ -183,10 +187,9 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
             mbar_init(op_empty(s), 1);
         }
         for (int b = 0; b < 2; ++b) {
-            mbar_init(lead_full(b), 1);
-            mbar_init(lead_empty(b), 4);
+            mbar_init(acc_full(b), 1);
+            mbar_init(acc_empty(b), 4);
         }
-        mbar_init(all_done, 1);
         mbar_init(drained, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -223,9 +226,8 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
         } else if (warp == 1 && lane == 0) {
             // -------------------------------------------------------- MMA
             // fp32 accumulator, bf16 operands (1), both MN-major, N >> 3, M >> 4
-            const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (1u << 16) | (8u << 24);
-            const uint32_t lead_desc = idesc | ((uint32_t)(p.nbp >> 3) << 17);
-            const uint32_t other_desc = idesc | ((uint32_t)(((PIECES - 1) * p.nbp) >> 3) << 17);
+            const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (1u << 16) |
+                                   ((uint32_t)((PIECES * p.nbp) >> 3) << 17) | (8u << 24);
             const uint64_t a_desc = smem_desc(base, 8192, 1024);
             const uint64_t b_desc = smem_desc(base + T * RA_BYTES, 8192, 1024);
             constexpr uint32_t step = 2048 >> 4;  // 16 rows of 128 bytes
@@ -234,7 +236,7 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
             bool ok = true;
             for (int kb = kb0; kb < kb1; ++kb) {
                 const int in_group = (kb - kb0) % RGROUP;
-                if (in_group == 0 && !mbar_wait_inline(lead_empty(b), bph ^ 1, p.status, 42)) { ok = false; break; }
+                if (in_group == 0 && !mbar_wait_inline(acc_empty(b), bph ^ 1, p.status, 42)) { ok = false; break; }
                 if (!mbar_wait_inline(op_full(s), ph, p.status, 43)) { ok = false; break; }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint64_t off = (uint64_t)((s * S::OP) >> 4);
@@ -243,25 +245,17 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
                     const uint64_t a = a_desc + off + (t * RA_BYTES >> 4), bb = b_desc + off;
 #pragma unroll
                     for (int k = 0; k < RK / 16; ++k)
-                        mma_f16(tmem + (b * T + t) * 64, a + step * k, bb + step * k, lead_desc,
+                        mma_f16(tmem + (b * T + t) * S::ACC, a + step * k, bb + step * k, idesc,
                                 (in_group > 0 || k > 0) ? 1u : 0u);
-                    if (PIECES > 1)
-#pragma unroll
-                        for (int k = 0; k < RK / 16; ++k)
-                            mma_f16(tmem + S::OTHER + t * 128, a + step * k, bb + (RB_BOX >> 4) + step * k, other_desc,
-                                    (kb > kb0 || k > 0) ? 1u : 0u);
                 }
                 mma_commit(op_empty(s));
                 if (++s == S::OPS) { s = 0; ph ^= 1; }
                 if (in_group == RGROUP - 1 || kb == kb1 - 1) {
-                    mma_commit(lead_full(b));
-                    b ^= 1;
-                    if (b == 0) bph ^= 1;
+                    mma_commit(acc_full(b));
+                    if (++b == S::BUFS) { b = 0; bph ^= 1; }
                 }
             }
-            if (ok) {
-                mma_commit(all_done);
-            } else {  // the MMAs in flight write TMEM: wait for them before it is freed
+            if (!ok) {  // the MMAs in flight write TMEM: wait for them before it is freed
                 mma_commit(drained);
                 mbar_drain_inline(drained, 0);
             }
@@ -280,50 +274,34 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
         uint32_t bph = 0;
         bool ok = true;
         for (int kb = kb0; kb < kb1; kb += RGROUP) {
-            bool got = true;
-            if (lane == 0) got = mbar_wait_inline(lead_full(b), bph, p.status, 44);
-            if (!__shfl_sync(FULL_WARP, got ? 1 : 0, 0)) { ok = false; break; }
+            if (!__all_sync(FULL_WARP, mbar_wait_inline(acc_full(b), bph, p.status, 44))) { ok = false; break; }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
             for (int t = 0; t < T; ++t)
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
                     if (16 * c < p.nbp) {
-                        uint32_t r[16];
-                        tmem_ld16_start(tl + (b * T + t) * 64 + 16 * c, r);
-                        tmem_ld16_wait(r);
+                        const uint32_t at = tl + (b * T + t) * S::ACC + 16 * c;
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) sum[t][16 * c + i] += __uint_as_float(r[i]);
-                    }
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            if (lane == 0) mbar_arrive(lead_empty(b));
-            b ^= 1;
-            if (b == 0) bph ^= 1;
-        }
-        if (ok) {  // every MMA is done: the others' accumulators are whole, the operand ring is free
-            bool got = true;
-            if (lane == 0) got = mbar_wait_inline(all_done, 0, p.status, 45);
-            ok = __shfl_sync(FULL_WARP, got ? 1 : 0, 0) != 0;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        }
-        if (ok) {
-            float* part = reinterpret_cast<float*>(smem);
-#pragma unroll
-            for (int t = 0; t < T; ++t) {
-                for (int q = PIECES - 1; q > 0; --q)
-#pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                        if (16 * c < p.nbp) {
+                        for (int q = PIECES - 1; q >= 0; --q) {  // the smallest piece first
                             uint32_t r[16];
-                            tmem_ld16_start(tl + S::OTHER + t * 128 + (q - 1) * p.nbp + 16 * c, r);
+                            tmem_ld16_start(at + q * p.nbp, r);
                             tmem_ld16_wait(r);
 #pragma unroll
                             for (int i = 0; i < 16; ++i) sum[t][16 * c + i] += __uint_as_float(r[i]);
                         }
+                    }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            if (lane == 0) mbar_arrive(acc_empty(b));
+            if (++b == S::BUFS) { b = 0; bph ^= 1; }
+        }
+        if (ok) {  // every MMA is done: the operand ring is free
+            float* part = reinterpret_cast<float*>(smem);
+#pragma unroll
+            for (int t = 0; t < T; ++t)
 #pragma unroll
                 for (int i = 0; i < 64; ++i)
                     if (i < p.nb) part[i * S::LD + t * 128 + quad * 32 + lane] = sum[t][i];
-            }
         }
     } else {
         // ------------------------------------------------------------ codes and U to bf16
@@ -337,8 +315,7 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
         const int units = p.nbp >> 3;
         int ur[NU], have[NU];  // a unit's row in the warp's part and its columns that exist (0: no unit)
         const U* from[NU];
-        // where its pieces go in an operand slot: the leading ones fill the first box, the others the next
-        // two, end to end
+        // where its pieces go in an operand slot: piece after piece, end to end
         uint32_t u_to[NU][PIECES];
 #pragma unroll
         for (int i = 0; i < NU; ++i) {
@@ -348,7 +325,7 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
             from[i] = static_cast<const U*>(p.u) + (long)(r0 + ur[i]) * p.ldu + 8 * uj;
 #pragma unroll
             for (int piece = 0; piece < PIECES; ++piece) {
-                const int col8 = piece == 0 ? uj : 8 + (piece - 1) * units + uj;
+                const int col8 = piece * units + uj;
                 u_to[i][piece] = T * RA_BYTES + (col8 >> 3) * RB_BOX + q8_sw128(r0 + ur[i], col8 & 7);
             }
         }
@@ -385,11 +362,10 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
             for (int i = 0; i < NU; ++i) un[i].values(u[i]);
             if (kb + 1 < kb1) prefetch(kb + 1);
             if (kb + RAHEAD < kb1) call(kb + RAHEAD);
-            bool got = true;
-            if (lane == 0)
-                got = mbar_wait_inline(op_empty(o), oph ^ 1, p.status, 46) &&
-                      mbar_wait_inline(raw_full(s), ph, p.status, 47);
-            if (!__shfl_sync(FULL_WARP, got ? 1 : 0, 0)) break;
+            // every lane waits (a lane that waited for its warp would cost the warp a detour); they agree
+            const bool got = mbar_wait_inline(op_empty(o), oph ^ 1, p.status, 46) &&
+                             mbar_wait_inline(raw_full(s), ph, p.status, 47);
+            if (!__all_sync(FULL_WARP, got)) break;
             unsigned char* op = smem + o * S::OP;
             const unsigned char* rw = smem + S::RAW_OFF + s * S::RAW;
             uint2 w[RROWS / RPP];
@@ -480,7 +456,7 @@ int clusters_at_once(int splits) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(1, (unsigned)splits, 1);
     cfg.blockDim = dim3(RTHREADS, 1, 1);
-    cfg.dynamicSmemBytes = RShape<T>::SMEM;
+    cfg.dynamicSmemBytes = RShape<T, Pieces<U>::N>::SMEM;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 1;
@@ -498,7 +474,7 @@ int clusters_at_once(int splits) {
 
 template <int T, bool E4M3, typename U>
 void launch(const RankCkpt8& a, RParams p, cudaStream_t s) {
-    typedef RShape<T> S;
+    typedef RShape<T, Pieces<U>::N> S;
     static DeviceOnce once;
     once([] {
         cudaFuncSetAttribute(rank_kernel<T, E4M3, U>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
