@@ -50,6 +50,34 @@ inline int current_sm_count() {
     return n;
 }
 
+// How many clusters of `size` CTAs of a kernel run at once on the current device: the GPU's
+// processing clusters differ in size, so this is not the SM count over the size.  `known` is the
+// caller's own cache for this kernel and size, one entry per device ordinal.
+template <typename Kernel>
+inline int clusters_at_once(Kernel* kern, int threads, size_t smem, int size, std::atomic<int> (&known)[64]) {
+    int dev = 0, n = 0;
+    const bool cached = cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64;
+    if (cached && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)size, 1, 1);
+    cfg.blockDim = dim3((unsigned)threads, 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)size;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n < 1) {
+        cudaGetLastError();
+        return 1;
+    }
+    if (cached) known[dev].store(n, std::memory_order_relaxed);
+    return n;
+}
+
 // A&S 7.1.26 GELU and the derivative of that approximation (the reference trains through
 // the approximation, src/ac/lora.h:97-110, so its gradient is the one autodiff yields).
 // The reciprocal and exponential use the fast hardware approximations (relative error ~1e-6):

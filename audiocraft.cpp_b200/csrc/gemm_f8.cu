@@ -21,6 +21,8 @@
 // X, which is a fixed permutation of the block's k that both operands share.
 #include <cuda.h>
 
+#include <atomic>
+
 #include "ckpt8.cuh"
 #include "tc_common.cuh"
 
@@ -35,6 +37,8 @@ constexpr int BM = 128, BK = 128;
 constexpr int A_BYTES = BM * BK;
 constexpr int NTHREADS = 384;  // four warps that feed, eight that add
 constexpr int ADDERS = 8;
+constexpr int SPLIT_LD = 128 + 4;  // floats of a row of a slice's sums
+constexpr int MAX_SPLIT = 8;       // portable cluster size
 // Scales of a k-block (128 of X, two of W) lie in a ring of their own: a slot is written when its
 // stage is, at most STAGES blocks ahead of the MMAs, and read at most two blocks (the TMEM
 // buffers) behind them, so that it is not overwritten before STAGES + 2 blocks have passed.
@@ -64,6 +68,7 @@ struct Params {
     int nk;           // k-blocks
     int mt, nt;       // tiles
     int dm, dn;       // the grid's stride over them
+    int splits;       // SPLIT: CTAs (a cluster) that share a tile's k-blocks
     const float *sx, *sw;
     long ldsx, ldsw;
     int sx_vec;       // X's scales move four at a time
@@ -159,11 +164,20 @@ __device__ __forceinline__ void put16(const Params& p, long at, long n, float v[
 }
 
 // the tiles of one CTA, column tiles first: CTAs that run together share rows of X
+template <bool SPLIT>
 struct Walk {
     int m, n;
-    __device__ __forceinline__ explicit Walk(const Params& p) : m(blockIdx.x / p.nt), n(blockIdx.x % p.nt) {}
+    __device__ __forceinline__ explicit Walk(const Params& p) {
+        const int first = SPLIT ? blockIdx.x / p.splits : blockIdx.x;
+        m = first / p.nt;
+        n = first % p.nt;
+    }
     __device__ __forceinline__ bool any(const Params& p) const { return m < p.mt; }
     __device__ __forceinline__ void next(const Params& p) {
+        if (SPLIT) {
+            m = p.mt;
+            return;
+        }
         m += p.dm;
         n += p.dn;
         if (n >= p.nt) {
@@ -173,7 +187,8 @@ struct Walk {
     }
 };
 
-template <int BN, bool MN>
+// SPLIT: a CTA has one tile, and its slice of the k-blocks
+template <int BN, bool MN, bool SPLIT>
 __global__ void __launch_bounds__(NTHREADS, 1) gemm_f8_kernel(const __grid_constant__ Maps maps, const Params p) {
     typedef Shape<BN> S;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -213,6 +228,9 @@ __global__ void __launch_bounds__(NTHREADS, 1) gemm_f8_kernel(const __grid_const
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *tmem_slot;
+    const int rank = SPLIT ? (int)cluster_ctarank() : 0;
+    const int kb0 = SPLIT ? (int)((long)p.nk * rank / p.splits) : 0;
+    const int kb1 = SPLIT ? (int)((long)p.nk * (rank + 1) / p.splits) : p.nk;
 
     // Registers: the four feeding warps give theirs to the eight that hold the sums (launched with
     // 168 each: 128 * 56 + 256 * 224 = 384 * 168).
@@ -224,9 +242,9 @@ __global__ void __launch_bounds__(NTHREADS, 1) gemm_f8_kernel(const __grid_const
             uint32_t ph = 0;
             long issued = 0;
             bool ok = true;
-            for (Walk t(p); ok && t.any(p); t.next(p)) {
+            for (Walk<SPLIT> t(p); ok && t.any(p); t.next(p)) {
                 const int m0 = t.m * BM, n0 = t.n * BN;
-                for (int kb = 0; kb < p.nk; ++kb, ++issued) {
+                for (int kb = kb0; kb < kb1; ++kb, ++issued) {
                     if (!mbar_wait_inline(empty_bar(s), ph ^ 1, p.status, 31)) { ok = false; break; }
                     const uint32_t sa = base + s * S::STAGE, sb = sa + A_BYTES;
                     mbar_expect_tx(full_bar(s), S::STAGE);
@@ -252,14 +270,14 @@ __global__ void __launch_bounds__(NTHREADS, 1) gemm_f8_kernel(const __grid_const
             uint32_t ph = 0;
             bool ok = true;
             const uint32_t ring = base + S::SCALE_OFF;
-            for (Walk t(p); ok && t.any(p); t.next(p)) {
+            for (Walk<SPLIT> t(p); ok && t.any(p); t.next(p)) {
                 // rows 4 lane .. 4 lane + 3 of X, and (lanes 0, 1) 128 columns of W each
                 const long m = (long)t.m * BM + 4 * lane, n = (long)t.n * BN + 128 * lane;
                 const bool whole = p.sx_vec && m + 4 <= p.M, w = lane < BN / 128 && n < p.N;
-                const float* sx = p.sx + m;
+                const float* sx = p.sx + (long)kb0 * p.ldsx + m;
                 // W's scales: [k-block][n-block], or [n-block][k-block] of a weight stored [K][N]
-                const float* sw = p.sw + (w ? (MN ? n / 128 * p.ldsw : n / 128) : 0);
-                for (int kb = 0; kb < p.nk; ++kb) {
+                const float* sw = p.sw + (w ? (MN ? n / 128 * p.ldsw : n / 128) : 0) + (long)kb0 * (MN ? 1 : p.ldsw);
+                for (int kb = kb0; kb < kb1; ++kb) {
                     if (!__all_sync(FULL_WARP, mbar_wait_inline(empty_bar(s), ph ^ 1, p.status, 35))) { ok = false; break; }
                     const uint32_t to = ring + slot * SCALE_LD * 4;
                     if (whole) {
@@ -291,8 +309,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) gemm_f8_kernel(const __grid_const
             int s = 0, b = 0;
             uint32_t ph = 0, bph = 0;
             bool ok = true;
-            for (Walk t(p); ok && t.any(p); t.next(p)) {
-                for (int kb = 0; kb < p.nk; ++kb) {
+            for (Walk<SPLIT> t(p); ok && t.any(p); t.next(p)) {
+                for (int kb = kb0; kb < kb1; ++kb) {
                     if (!mbar_wait_inline(tempty(b), bph ^ 1, p.status, 32) ||
                         !mbar_wait_inline(full_bar(s), ph, p.status, 33)) {
                         ok = false;
@@ -325,12 +343,12 @@ __global__ void __launch_bounds__(NTHREADS, 1) gemm_f8_kernel(const __grid_const
         int b = 0;
         uint32_t bph = 0;
         bool ok = true;
-        for (Walk w(p); ok && w.any(p); w.next(p)) {
+        for (Walk<SPLIT> w(p); ok && w.any(p); w.next(p)) {
             const long m0 = (long)w.m * BM + quad * 32, n0 = (long)w.n * BN + half * S::HALF;
             uint64_t acc[S::HALF / 2];
 #pragma unroll
             for (int i = 0; i < S::HALF / 2; ++i) acc[i] = 0;
-            for (int kb = 0; kb < p.nk; ++kb) {
+            for (int kb = kb0; kb < kb1; ++kb) {
                 // every lane waits (a lane that waited for its warp would cost the warp a detour); they agree
                 if (!__all_sync(FULL_WARP, mbar_wait_inline(tfull(b), bph, p.status, 34))) { ok = false; break; }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -356,6 +374,15 @@ __global__ void __launch_bounds__(NTHREADS, 1) gemm_f8_kernel(const __grid_const
                 if (b == 0) bph ^= 1;
             }
             if (!ok) break;
+            if (SPLIT) {  // this slice's sums, where the operand ring was: every MMA that read it is done
+                float* to = reinterpret_cast<float*>(smem) + (quad * 32 + lane) * SPLIT_LD + half * S::HALF;
+#pragma unroll
+                for (int i = 0; i < S::HALF / 4; ++i) {
+                    const float2 u = unpair(acc[2 * i]), v = unpair(acc[2 * i + 1]);
+                    *reinterpret_cast<float4*>(to + 4 * i) = make_float4(u.x, u.y, v.x, v.y);
+                }
+                break;
+            }
             // epilogue: a row per thread, 16 columns at a time
             const long m = m0 + lane;
             if (m < p.M) {
@@ -378,6 +405,37 @@ __global__ void __launch_bounds__(NTHREADS, 1) gemm_f8_kernel(const __grid_const
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (warp == 0)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::TMEM));
+    if (SPLIT) {
+        // every thread of every CTA of the cluster passes both barriers
+        cluster_sync_all();
+        const Walk<SPLIT> w(p);
+        constexpr int G = BN / 4;  // groups of 4 columns of a row
+        const int r0 = BM * rank / p.splits, r1 = BM * (rank + 1) / p.splits;
+        for (int i = threadIdx.x; i < (r1 - r0) * G; i += NTHREADS) {
+            const int r = r0 + i / G, c = i % G * 4;
+            const long m = (long)w.m * BM + r, n = (long)w.n * BN + c;
+            if (m >= p.M || n >= p.N) continue;
+            const uint32_t at = base + (uint32_t)(r * SPLIT_LD + c) * 4;
+            float4 d[MAX_SPLIT];  // all under way together
+#pragma unroll
+            for (int q = 0; q < MAX_SPLIT; ++q)
+                if (q < p.splits) d[q] = ld_dsmem_f4(map_cta(at, (uint32_t)q));
+            float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int q = 0; q < MAX_SPLIT; ++q)  // slice order: the same sum whoever finished first
+                if (q < p.splits) {
+                    v[0] += d[q].x; v[1] += d[q].y; v[2] += d[q].z; v[3] += d[q].w;
+                }
+            const long o = m * p.ldy + n;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (n + j < p.N) {
+                    const float s = v[j] + (p.bias ? __ldg(p.bias + n + j) : 0.f);
+                    put_value(p, o + j, p.accumulate ? old_value(p, o + j) + s : s);
+                }
+        }
+        cluster_sync_all();  // peers keep their sums until every reader is done
+    }
 }
 
 // ---------------------------------------------------------------------------------------
@@ -465,12 +523,13 @@ __global__ void __launch_bounds__(SM_WARPS * 32) gemm_f8_small_kernel(const uint
     }
 }
 
-template <int BN, bool MN>
+template <int BN, bool MN, bool SPLIT>
 void launch(const GemmF8& a, Params p, cudaStream_t s) {
     typedef Shape<BN> S;
+    static_assert(!SPLIT || (BN == 128 && BM * SPLIT_LD * 4 <= S::STAGES * S::STAGE), "a slice's sums take the ring's place");
     static DeviceOnce once;
     once([] {
-        cudaFuncSetAttribute(gemm_f8_kernel<BN, MN>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+        cudaFuncSetAttribute(gemm_f8_kernel<BN, MN, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
     });
     Maps maps;
     tc_make_map_u8(&maps.x, a.x.q, a.M, a.K, a.x.ldq, BK, BM);
@@ -479,16 +538,46 @@ void launch(const GemmF8& a, Params p, cudaStream_t s) {
     p.mt = (int)((a.M + BM - 1) / BM);
     p.nt = (int)((a.N + BN - 1) / BN);
     const long tiles = (long)p.mt * p.nt, sms = current_sm_count();
-    const int ctas = (int)(tiles < sms ? tiles : sms);
+    const int ctas = SPLIT ? (int)tiles * p.splits : (int)(tiles < sms ? tiles : sms);
     p.dm = ctas / p.nt;
     p.dn = ctas % p.nt;
-    gemm_f8_kernel<BN, MN><<<(unsigned)ctas, NTHREADS, S::SMEM, s>>>(maps, p);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)ctas, 1, 1);
+    cfg.blockDim = dim3(NTHREADS, 1, 1);
+    cfg.dynamicSmemBytes = S::SMEM;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = SPLIT ? (unsigned)p.splits : 1;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, gemm_f8_kernel<BN, MN, SPLIT>, maps, p);
 }
 
-template <int BN>
+template <int BN, bool SPLIT>
 void launch(const GemmF8& a, const Params& p, cudaStream_t s) {
-    if (a.w_mn) launch<BN, true>(a, p, s);
-    else launch<BN, false>(a, p, s);
+    if (a.w_mn) launch<BN, true, SPLIT>(a, p, s);
+    else launch<BN, false, SPLIT>(a, p, s);
+}
+
+// CTAs per tile for a product of few tiles: the least rounds of clusters times the k-blocks of a
+// slice and what joining the slices costs, about as long as twelve k-blocks
+template <bool MN>
+int best_split(long tiles, int nk) {
+    static std::atomic<int> known[MAX_SPLIT + 1][64];
+    int splits = 1;
+    long best = nk;
+    for (int n = 2; n <= MAX_SPLIT && n <= nk; ++n) {
+        const long at_once = clusters_at_once(gemm_f8_kernel<128, MN, true>, NTHREADS, Shape<128>::SMEM, n, known[n]);
+        const long cost = (tiles + at_once - 1) / at_once * ((nk + n - 1) / n + 12);
+        if (cost < best) {
+            best = cost;
+            splits = n;
+        }
+    }
+    return splits;
 }
 
 }  // namespace
@@ -501,17 +590,22 @@ void gemm_f8(const GemmF8& a, cudaStream_t s) {
     p.bias = a.bias; p.y = const_cast<void*>(a.y.p); p.y_type = a.y.type; p.accumulate = a.accumulate ? 1 : 0;
     p.ldy = a.y.ld; p.vec = a.y.ld * op_bytes(a.y.type) % 32 == 0 && reinterpret_cast<uintptr_t>(a.y.p) % 32 == 0 && vec4(a.bias); p.status = a.status;
     p.mt = p.nt = p.dm = p.dn = 0;
+    p.splits = 1;
     if (a.M <= SM_MAX_M && !a.w_mn) {
         const unsigned ctas = (unsigned)((a.N + SM_ROWS - 1) / SM_ROWS);
         if (a.M <= 8) gemm_f8_small_kernel<1><<<ctas, SM_WARPS * 32, 0, s>>>(a.x.q, a.x.ldq, a.w.q, a.w.ldq, p);
         else gemm_f8_small_kernel<2><<<ctas, SM_WARPS * 32, 0, s>>>(a.x.q, a.x.ldq, a.w.q, a.w.ldq, p);
         return;
     }
+    const long mt = (a.M + BM - 1) / BM, sms = current_sm_count(), narrow = mt * ((a.N + 127) / 128);
+    if (narrow < sms) {
+        p.splits = a.w_mn ? best_split<true>(narrow, p.nk) : best_split<false>(narrow, p.nk);
+        if (p.splits > 1) return launch<128, true>(a, p, s);
+    }
     // 256-wide tiles unless 128-wide ones finish in fewer column-rounds over the SMs
-    const long mt = (a.M + BM - 1) / BM, sms = current_sm_count();
     auto cost = [&](long bn) { return (mt * ((a.N + bn - 1) / bn) + sms - 1) / sms * bn; };
-    if (cost(128) < cost(256)) launch<128>(a, p, s);
-    else launch<256>(a, p, s);
+    if (cost(128) < cost(256)) launch<128, false>(a, p, s);
+    else launch<256, false>(a, p, s);
 }
 
 }  // namespace act

@@ -5,7 +5,7 @@
 // codes into tensor-core operands keeps up.  A CTA owns 128 or 256 columns of X (the rows of the MMA)
 // and a slice of the rows t (the reduction), in blocks of 64:
 //   warp 0     TMA: raw codes into a ring of 64-row blocks
-//   warps 8-23 codes * scale -> bf16 (exact: 4 or 7 significant bits times a power of two) in the
+//   warps 8-15 codes * scale -> bf16 (exact: 4 or 7 significant bits times a power of two) in the
 //              128-byte-swizzled MN-major layout; the block's rows of U, cut into bf16 pieces that add
 //              up to it exactly (one for bf16, two for f16, three for fp32): both operands of the
 //              MMA have to be bf16, and the product keeps all of U
@@ -34,8 +34,7 @@ using namespace tc;
 
 constexpr int RK = 64;                   // rows t of a block
 constexpr int RGROUP = 4;                // blocks between two emptyings of the accumulators
-constexpr int RCONV = 16;                // converting warps
-constexpr int RAHEAD = 8;
+constexpr int RCONV = 8;                 // converting warps
 constexpr int RROWS = RK / RCONV;        // rows of a block each takes
 constexpr int RTHREADS = (8 + RCONV) * 32;
 constexpr int RA_BYTES = 128 * RK * 2;   // bf16 operand of 128 columns
@@ -204,9 +203,9 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *tmem_slot;
 
-    // Launched with 80 registers a thread: 40 + 152 + 4 * 72 = 6 * 80.
+    // Launched with 128 registers a thread: 56 + 152 + 2 * 152 = 4 * 128.
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (warp == 0 && lane == 0) {
             // -------------------------------------------------------- TMA
             int s = 0, issued = 0;
@@ -305,7 +304,7 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
         }
     } else {
         // ------------------------------------------------------------ codes and U to bf16
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
         constexpr int LPR = 16 * T;        // lanes of a row (8 codes each)
         constexpr int RPP = 32 / LPR;      // rows of a pass
         const int cw = warp - 8, r0 = RROWS * cw;  // rows r0 .. r0 + RROWS - 1 of each block
@@ -341,17 +340,6 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
                 un[i].load(from[i] + (long)kb * RK * p.ldu, t0 + ur[i] < p.rows ? have[i] : 0, p.u_vec);
             sn = fetch && t0 + lane % RROWS < p.rows ? scales[t0] : 0.f;
         };
-        // U and the scales come straight to registers one block ahead, which covers L2's latency but not
-        // HBM's: they are called into L2 RAHEAD blocks before that
-        auto call = [&](int kb) {
-            const int t0 = kb * RK + r0;
-#pragma unroll
-            for (int i = 0; i < NU; ++i)
-                if (have[i] > 0 && t0 + ur[i] < p.rows)
-                    asm volatile("prefetch.global.L2 [%0];" ::"l"(from[i] + (long)kb * RK * p.ldu));
-            if (fetch && t0 + lane % RROWS < p.rows) asm volatile("prefetch.global.L2 [%0];" ::"l"(scales + t0));
-        };
-        for (int kb = kb0; kb < kb0 + RAHEAD && kb < kb1; ++kb) call(kb);
         if (kb0 < kb1) prefetch(kb0);
         int s = 0, o = 0;
         uint32_t ph = 0, oph = 0;
@@ -361,7 +349,6 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
 #pragma unroll
             for (int i = 0; i < NU; ++i) un[i].values(u[i]);
             if (kb + 1 < kb1) prefetch(kb + 1);
-            if (kb + RAHEAD < kb1) call(kb + RAHEAD);
             // every lane waits (a lane that waited for its warp would cost the warp a detour); they agree
             const bool got = mbar_wait_inline(op_empty(o), oph ^ 1, p.status, 46) &&
                              mbar_wait_inline(raw_full(s), ph, p.status, 47);
@@ -421,11 +408,16 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
         const long c = c0 + f;
         if (c >= p.cols) continue;
         const uint32_t at = part + (uint32_t)(j * S::LD + f) * 4;
+        float4 d[RMAX_SPLIT];  // all under way together
+#pragma unroll
+        for (int q = 0; q < RMAX_SPLIT; ++q)
+            if (q < p.splits) d[q] = ld_dsmem_f4(p.splits > 1 ? map_cta(at, (uint32_t)q) : at);
         float v[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int q = 0; q < p.splits; ++q) {  // slice order: the same sum whoever finished first
-            const float4 d = ld_dsmem_f4(p.splits > 1 ? map_cta(at, (uint32_t)q) : at);
-            v[0] += d.x; v[1] += d.y; v[2] += d.z; v[3] += d.w;
-        }
+#pragma unroll
+        for (int q = 0; q < RMAX_SPLIT; ++q)  // slice order: the same sum whoever finished first
+            if (q < p.splits) {
+                v[0] += d[q].x; v[1] += d[q].y; v[2] += d[q].z; v[3] += d[q].w;
+            }
         float* out = p.c + j * p.ldc + c;
 #pragma unroll
         for (int k = 0; k < 4; ++k) v[k] *= p.alpha;
@@ -443,35 +435,6 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
     if (p.splits > 1) cluster_sync_all();  // peers keep their sums until every reader is done
 }
 
-// How many clusters of `splits` CTAs run at once on the current device: the GPU's processing
-// clusters differ in size, so this is not the SM count over the size.  Asked once per device.
-template <int T, bool E4M3, typename U>
-int clusters_at_once(int splits) {
-    static std::atomic<int> known[64][RMAX_SPLIT + 1];
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return 1;
-    const bool cached = dev >= 0 && dev < 64;
-    int n = cached ? known[dev][splits].load(std::memory_order_relaxed) : 0;
-    if (n > 0) return n;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(1, (unsigned)splits, 1);
-    cfg.blockDim = dim3(RTHREADS, 1, 1);
-    cfg.dynamicSmemBytes = RShape<T, Pieces<U>::N>::SMEM;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 1;
-    attr[0].val.clusterDim.y = (unsigned)splits;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    if (cudaOccupancyMaxActiveClusters(&n, rank_kernel<T, E4M3, U>, &cfg) != cudaSuccess || n < 1) {
-        cudaGetLastError();
-        return 1;
-    }
-    if (cached) known[dev][splits].store(n, std::memory_order_relaxed);
-    return n;
-}
-
 template <int T, bool E4M3, typename U>
 void launch(const RankCkpt8& a, RParams p, cudaStream_t s) {
     typedef RShape<T, Pieces<U>::N> S;
@@ -482,9 +445,10 @@ void launch(const RankCkpt8& a, RParams p, cudaStream_t s) {
     const long tiles = (a.cols + T * 128 - 1) / (T * 128);
     // slices per tile: the least rounds of clusters times blocks of a slice
     p.splits = 1;
+    static std::atomic<int> known[RMAX_SPLIT + 1][64];
     long best = -1;
     for (int n = 1; n <= RMAX_SPLIT && n <= p.nk; ++n) {
-        const long at_once = clusters_at_once<T, E4M3, U>(n);
+        const long at_once = clusters_at_once(rank_kernel<T, E4M3, U>, RTHREADS, S::SMEM, n, known[n]);
         const long cost = (tiles + at_once - 1) / at_once * ((p.nk + n - 1) / n);
         if (best < 0 || cost < best) {
             best = cost;
