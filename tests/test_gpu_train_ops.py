@@ -573,6 +573,16 @@ def test_gemm(M, N, K, mn):
         assert y.untouched() and st.item() == 0
 
 
+# few tiles and many k-blocks: clusters share a tile's reduction (slices of unequal length, a ragged last one)
+FEW_TILES = [(20, 130, 4100), (130, 256, 6144), (100, 1000, 3001), (257, 129, 2600)]
+
+
+@pytest.mark.parametrize("M,N,K", FEW_TILES)
+@pytest.mark.parametrize("mn", [False, True], ids=["k_major", "mn_major"])
+def test_gemm_of_few_tiles(M, N, K, mn):
+    test_gemm(M, N, K, mn)
+
+
 def test_gemm_takes_any_scale_and_keeps_nan_in_its_place():
     rng = np.random.default_rng(4)
     for M in (5, 200):
@@ -605,6 +615,89 @@ def test_gemm_with_a_scale_table_that_underflows():
     A.gemm_f8(x.v, w.v, M, N, K, y.ptr, A.TYPE_F16, st.data_ptr(), stream=stream())
     torch.cuda.synchronize()
     assert np.all(y.np() == 0)
+
+
+# ------------------------------------------------------------------------------ far offsets
+def far(rows, ld, dtype):
+    return torch.empty((rows - 1) * ld + 512, dtype=dtype, device="cuda")
+
+
+def rows_of(buf, rows, cols, ld):
+    return buf.as_strided((rows, cols), (ld, 1))
+
+
+def test_rows_more_than_32_bits_apart():
+    # strides of 1.5 G elements: row 2 starts beyond 2^31 elements and 2^32 bytes
+    rows, cols, ld = 3, 300, 1_500_000_000
+    rng = np.random.default_rng(5)
+    X = rounded(rng.standard_normal((rows, cols)), "bf16")
+    x, q, y = far(rows, ld, torch.bfloat16), far(rows, ld, torch.uint8), far(rows, ld, torch.bfloat16)
+    rows_of(x, rows, cols, ld).copy_(torch.from_numpy(X))
+    scale = torch.zeros(3, rows, device="cuda")
+    v = A.ckpt8(A.CKPT_E4M3, q.data_ptr(), ld, scale.data_ptr(), rows)
+    A.ckpt8_store(x.data_ptr(), A.TYPE_BF16, rows, cols, v, ldx=ld, stream=stream())
+    A.ckpt8_load(v, rows, cols, y.data_ptr(), A.TYPE_BF16, ldy=ld, stream=stream())
+    torch.cuda.synchronize()
+    want = E.decode(*E.encode(X, A.CKPT_E4M3), A.CKPT_E4M3)
+    np.testing.assert_array_equal(rows_of(y, rows, cols, ld).double().cpu().numpy(), want)
+    # norm there and back, GELU there and back, all through the far rows
+    st, sums = torch.zeros(2, rows, device="cuda"), torch.zeros(2, cols, device="cuda")
+    A.layernorm_fwd(x.data_ptr(), A.TYPE_BF16, rows, cols, 0, 0, y.data_ptr(), A.TYPE_BF16, st[0].data_ptr(),
+                    st[1].data_ptr(), ldx=ld, ldy=ld, stream=stream())
+    torch.cuda.synchronize()
+    mean, rstd = E.norm_stats(X, 1e-5)
+    H = (X - mean[:, None]) * rstd[:, None]
+    np.testing.assert_allclose(rows_of(y, rows, cols, ld).double().cpu().numpy(), H, rtol=2.0 ** -7, atol=1e-5)
+    room = A.layernorm_bwd_workspace(rows, cols)
+    space = torch.empty(room // 4, device="cuda")
+    A.layernorm_bwd(x.data_ptr(), A.TYPE_BF16, 0, 0, 0, st[0].data_ptr(), st[1].data_ptr(), rows, cols, y.data_ptr(),
+                    A.TYPE_BF16, sums[0].data_ptr(), sums[1].data_ptr(), space.data_ptr(), room, x8=v, lddy=ld,
+                    lddx=ld, stream=stream())
+    torch.cuda.synchronize()
+    dx, dw, db = E.norm_back(X, want, np.ones((1, cols)), mean, rstd)
+    np.testing.assert_allclose(rows_of(y, rows, cols, ld).double().cpu().numpy(), dx, rtol=2.0 ** -7, atol=1e-4)
+    np.testing.assert_allclose(sums[1].double().cpu().numpy(), db, atol=1e-5)
+    A.gelu_ckpt8_fwd(x.data_ptr(), A.TYPE_BF16, rows, cols, y.data_ptr(), A.TYPE_BF16, v, ldz=ld, ldg=ld,
+                     stream=stream())
+    torch.cuda.synchronize()
+    np.testing.assert_allclose(rows_of(y, rows, cols, ld).double().cpu().numpy(), E.gelu(X), rtol=2.0 ** -7, atol=1e-5)
+    A.gelu_ckpt8_bwd(x.data_ptr(), A.TYPE_BF16, v, rows, cols, y.data_ptr(), A.TYPE_BF16, lddg=ld, lddz=ld,
+                     stream=stream())
+    torch.cuda.synchronize()
+    np.testing.assert_allclose(rows_of(y, rows, cols, ld).double().cpu().numpy(), X * E.gelu_grad(want),
+                               rtol=2.0 ** -7, atol=1e-5)
+    # products: C and Y with far rows, X with far rows
+    u = torch.from_numpy(X[:, :3].copy()).to("cuda").float()
+    word, c = status_word(), far(3, ld, torch.float32)
+    A.ckpt8_store(x.data_ptr(), A.TYPE_BF16, rows, cols, v, ldx=ld, stream=stream())
+    A.rank_gemm_ckpt8(u.data_ptr(), A.TYPE_F32, 3, v, rows, cols, c.data_ptr(), word.data_ptr(), ldc=ld,
+                      stream=stream())
+    torch.cuda.synchronize()
+    np.testing.assert_allclose(rows_of(c, 3, cols, ld).double().cpu().numpy(), X[:, :3].T @ want, atol=1e-5)
+    del c
+    w = Eight(40, cols, A.CKPT_E4M3, 128, up16(cols), data=E.encode(rng.standard_normal((40, cols)), A.CKPT_E4M3, 128))
+    out = far(rows, ld, torch.bfloat16)
+    A.gemm_f8(v, w.v, rows, 40, cols, out.data_ptr(), A.TYPE_BF16, word.data_ptr(), ldy=ld, stream=stream())
+    torch.cuda.synchronize()
+    np.testing.assert_allclose(rows_of(out, rows, 40, ld).double().cpu().numpy(), want @ w.np().T, rtol=2.0 ** -7,
+                               atol=1e-4)
+
+
+def test_gemm_of_rows_more_than_32_bits_apart_on_the_tensor_cores():
+    rows, cols, ld = 200, 256, 1 << 25
+    rng = np.random.default_rng(6)
+    qx, sx = E.encode(rng.standard_normal((rows, cols)), A.CKPT_E4M3)
+    q = far(rows, ld, torch.uint8)
+    rows_of(q, rows, cols, ld).copy_(torch.from_numpy(qx))
+    scale = torch.from_numpy(sx.astype(np.float32)).to("cuda")
+    v = A.ckpt8(A.CKPT_E4M3, q.data_ptr(), ld, scale.data_ptr(), rows)
+    w = Eight(300, cols, A.CKPT_E4M3, 128, up16(cols), data=E.encode(rng.standard_normal((300, cols)), A.CKPT_E4M3, 128))
+    y, word = out_mat(rows, 300, "f32"), status_word()
+    A.gemm_f8(v, w.v, rows, 300, cols, y.ptr, A.TYPE_F32, word.data_ptr(), stream=stream())
+    torch.cuda.synchronize()
+    X = E.decode(qx, sx, A.CKPT_E4M3)
+    assert_close(y.np(), X @ w.np().T, (2 * cols + 6) * U * (np.abs(X) @ np.abs(w.np()).T), "far")
+    assert word.item() == 0
 
 
 # ------------------------------------------------------------------------------ how they are called
