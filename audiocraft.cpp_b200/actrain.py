@@ -522,73 +522,84 @@ def ckpt8(type: int, q: int, ldq: int, scale: int, lds: int) -> Ckpt8:
     return Ckpt8(type, q, ldq, scale, lds)
 
 
-def _call(rc):
-    if rc != ACT_OK:
-        raise ActError(rc, lib().act_last_error(None).decode())
-
-
-def _ref(view):
-    return None if view is None else C.byref(view)
+def _failed(rc):
+    raise ActError(rc, lib().act_last_error(None).decode())
 
 
 def ckpt8_store(x, x_type, rows, cols, out, block_rows=1, ldx=0, stream=0):
     """act_ckpt8_store: x [rows][cols] in 8 bits, blocks of 128 columns x block_rows (1 or 128) rows."""
-    _call(lib().act_ckpt8_store(x, x_type, ldx or cols, rows, cols, block_rows, _ref(out), stream))
+    rc = (_lib or lib()).act_ckpt8_store(x, x_type, ldx or cols, rows, cols, block_rows, out, stream)
+    if rc:
+        _failed(rc)
 
 
 def ckpt8_load(src, rows, cols, y, y_type, block_rows=1, ldy=0, stream=0):
     """act_ckpt8_load: the values an 8-bit tensor stands for, rounded to y_type."""
-    _call(lib().act_ckpt8_load(_ref(src), rows, cols, block_rows, y, y_type, ldy or cols, stream))
+    rc = (_lib or lib()).act_ckpt8_load(src, rows, cols, block_rows, y, y_type, ldy or cols, stream)
+    if rc:
+        _failed(rc)
 
 
 def layernorm_fwd(x, x_type, rows, dim, w, b, y, y_type, mean, rstd, eps=1e-5, ldx=0, ldy=0, y8=None, x8=None,
                   stream=0):
     """act_layernorm_fwd: y (and y8, its 8-bit form), row statistics, and x8, the 8-bit checkpoint of x."""
-    _call(lib().act_layernorm_fwd(x, x_type, ldx or dim, rows, dim, w, b, eps, y, y_type, ldy or dim, _ref(y8), mean,
-                                  rstd, _ref(x8), stream))
+    rc = (_lib or lib()).act_layernorm_fwd(x, x_type, ldx or dim, rows, dim, w, b, eps, y, y_type, ldy or dim, y8, mean,
+                                           rstd, x8, stream)
+    if rc:
+        _failed(rc)
 
 
 def layernorm_bwd_workspace(rows, dim) -> int:
     """Bytes of workspace act_layernorm_bwd needs for this shape on the current device."""
     n = int(lib().act_layernorm_bwd_workspace(rows, dim))
     if n < 0:
-        _call(ACT_ERR_INVALID)
+        _failed(ACT_ERR_INVALID)
     return n
 
 
 def layernorm_bwd(dy, dy_type, x, x_type, w, mean, rstd, rows, dim, dx, dx_type, dw, db, workspace, workspace_bytes,
                   accumulate=False, add=0, x8=None, lddy=0, ldx=0, lddx=0, stream=0):
     """act_layernorm_bwd: dx, and the sums over the rows dw and db; x = 0 reads the checkpoint x8 instead."""
-    _call(lib().act_layernorm_bwd(dy, dy_type, lddy or dim, x, x_type, ldx or dim, _ref(x8), w, mean, rstd, rows, dim,
-                                  add, dx, dx_type, lddx or dim, dw, db, int(accumulate), workspace, workspace_bytes,
-                                  stream))
+    rc = (_lib or lib()).act_layernorm_bwd(dy, dy_type, lddy or dim, x, x_type, ldx or dim, x8, w, mean, rstd, rows, dim,
+                                           add, dx, dx_type, lddx or dim, dw, db, int(accumulate), workspace, workspace_bytes,
+                                           stream)
+    if rc:
+        _failed(rc)
 
 
 def gelu_ckpt8_fwd(z, z_type, rows, cols, g, g_type, z8, g8=None, ldz=0, ldg=0, stream=0):
     """act_gelu_ckpt8_fwd: g (and g8) = GELU(z), z8 = the 8-bit checkpoint of z; g_type is z_type."""
     if g_type != z_type:
         raise ActError(ACT_ERR_INVALID, "gelu_ckpt8_fwd: g has z's type")
-    _call(lib().act_gelu_ckpt8_fwd(z, z_type, ldz or cols, rows, cols, g, ldg or cols, _ref(g8), _ref(z8), stream))
+    rc = (_lib or lib()).act_gelu_ckpt8_fwd(z, z_type, ldz or cols, rows, cols, g, ldg or cols, g8, z8, stream)
+    if rc:
+        _failed(rc)
 
 
 def gelu_ckpt8_bwd(dg, dg_type, z8, rows, cols, dz, dz_type, dz8=None, lddg=0, lddz=0, stream=0):
     """act_gelu_ckpt8_bwd: dz (and dz8) = dg * GELU'(kept z); dz_type is dg_type."""
     if dz_type != dg_type:
         raise ActError(ACT_ERR_INVALID, "gelu_ckpt8_bwd: dz has dg's type")
-    _call(lib().act_gelu_ckpt8_bwd(dg, dg_type, lddg or cols, _ref(z8), rows, cols, dz, lddz or cols, _ref(dz8),
-                                   stream))
+    rc = (_lib or lib()).act_gelu_ckpt8_bwd(dg, dg_type, lddg or cols, z8, rows, cols, dz, lddz or cols, dz8,
+                                            stream)
+    if rc:
+        _failed(rc)
 
 
 def rank_gemm_ckpt8(u, u_type, nb, x8, rows, cols, c, status, alpha=1.0, accumulate=False, ldu=0, ldc=0, stream=0):
     """act_rank_gemm_ckpt8: C [nb][cols] (+)= alpha * U^T X with X an 8-bit tensor [rows][cols]."""
-    _call(lib().act_rank_gemm_ckpt8(u, u_type, ldu or nb, nb, _ref(x8), rows, cols, alpha, c, ldc or cols,
-                                    int(accumulate), status, stream))
+    rc = (_lib or lib()).act_rank_gemm_ckpt8(u, u_type, ldu or nb, nb, x8, rows, cols, alpha, c, ldc or cols,
+                                             int(accumulate), status, stream)
+    if rc:
+        _failed(rc)
 
 
 def gemm_f8(x8, w8, M, N, K, y, y_type, status, w_mn_major=False, bias=0, accumulate=False, ldy=0, stream=0):
     """act_gemm_f8: Y [M][N] (+)= X8 W8^T (+ bias), W8 [N][K] or, with w_mn_major, [K][N]."""
-    _call(lib().act_gemm_f8(_ref(x8), _ref(w8), M, N, K, int(w_mn_major), bias, y, y_type, ldy or N, int(accumulate),
-                            status, stream))
+    rc = (_lib or lib()).act_gemm_f8(x8, w8, M, N, K, int(w_mn_major), bias, y, y_type, ldy or N, int(accumulate),
+                                     status, stream)
+    if rc:
+        _failed(rc)
 
 
 def mf_model(dim, layers, heads, ff_dim, latent_dim=128, cond_dim=768, time_dim=256, norm_eps=1e-5):
