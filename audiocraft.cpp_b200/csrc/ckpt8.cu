@@ -42,21 +42,25 @@ __device__ __forceinline__ Place place(long cols) {
 }
 
 // body(place, held, row, rows, whole) for each of the warp's groups of up to RPW rows; `held` is what
-// fetch(place, held, row, rows) has loaded of them, one group ahead of its use
+// fetch(place, held, row, rows, whole) has loaded of them, one group ahead of its use.  `whole` (a
+// type) says that all RPW rows exist, which saves the tests.
 template <bool VEC, typename Held, typename Fetch, typename Body>
 __device__ __forceinline__ void each_group(long rows, long cols, Fetch&& fetch, Body&& body) {
     const Place p = place<VEC>(cols);
     if (!p.any || p.row >= rows) return;
     Held next;
     long row = p.row;
-    auto count = [&](long r) { return rows - r < RPW ? (int)(rows - r) : RPW; };
-    fetch(p, next, row, count(row));
+    auto get = [&](long r) {
+        if (r + RPW <= rows) fetch(p, next, r, RPW, std::true_type());
+        else if (r < rows) fetch(p, next, r, (int)(rows - r), std::false_type());
+    };
+    get(row);
     for (; row + RPW <= rows; row += p.step) {
         const Held held = next;
-        if (row + p.step < rows) fetch(p, next, row + p.step, count(row + p.step));
+        get(row + p.step);
         body(p, held, row, RPW, std::true_type());
     }
-    if (row < rows) body(p, next, row, count(row), std::false_type());
+    if (row < rows) body(p, next, row, (int)(rows - row), std::false_type());
 }
 
 // the scales of up to RPW rows: lane r holds row r's
@@ -69,7 +73,7 @@ __device__ __forceinline__ void store_scales(const Q8& t, int chunk, long row, i
 }
 
 // v: RPW rows of a block, -> codes and scales
-template <bool VEC, bool FULL>
+template <bool VEC, bool WHOLE>
 __device__ __forceinline__ void store_rows(const Q8& t, const Place& p, long row, int nr, const float (*v)[4],
                                            bool e4m3) {
     uint32_t s[RPW], top[RPW], most = 0;
@@ -86,7 +90,7 @@ __device__ __forceinline__ void store_rows(const Q8& t, const Place& p, long row
 #pragma unroll
     for (int r = 0; r < RPW; ++r) {
         s[r] = scale_bits(top[r], e4m3);
-        store_codes<VEC>(q + r * t.ldq, FULL || r < nr ? p.n : 0, encode4(v[r], inverse_pow2(s[r]), e4m3, bad));
+        store_codes<VEC>(q + r * t.ldq, WHOLE || r < nr ? p.n : 0, encode4(v[r], inverse_pow2(s[r]), e4m3, bad));
     }
     store_scales(t, p.chunk, row, nr, s);
 }
@@ -94,9 +98,10 @@ __device__ __forceinline__ void store_rows(const Q8& t, const Place& p, long row
 template <typename T, bool VEC>
 struct HeldRows {
     Raw4<T, VEC> x[RPW];
+    template <bool WHOLE>
     __device__ __forceinline__ void load(const T* at, long ld, int n, int nr) {
 #pragma unroll
-        for (int r = 0; r < RPW; ++r) x[r].load(at + r * ld, r < nr ? n : 0);
+        for (int r = 0; r < RPW; ++r) x[r].load(at + r * ld, WHOLE || r < nr ? n : 0);
     }
 };
 
@@ -105,7 +110,9 @@ __global__ void __launch_bounds__(THREADS) store_kernel(const T* x, long ldx, lo
     typedef HeldRows<T, VEC> Held;
     each_group<VEC, Held>(
         rows, cols,
-        [&](const Place& p, Held& h, long row, int nr) { h.load(x + row * ldx + p.col, ldx, p.n, nr); },
+        [&](const Place& p, Held& h, long row, int nr, auto whole) {
+            h.template load<decltype(whole)::value>(x + row * ldx + p.col, ldx, p.n, nr);
+        },
         [&](const Place& p, const Held& h, long row, int nr, auto whole) {
             float v[RPW][4];
 #pragma unroll
@@ -172,13 +179,14 @@ struct HeldCodes {
     uint32_t w[RPW];
     float s[RPW];
     // shift: log2 of the block's rows
+    template <bool WHOLE>
     __device__ __forceinline__ void load(const Q8& t, const Place& p, long row, int nr, int shift) {
         const uint8_t* q = t.q + row * t.ldq + p.col;
         const float* scale = t.scale + (long)p.chunk * t.lds;
 #pragma unroll
         for (int r = 0; r < RPW; ++r) {
-            w[r] = load_codes<VEC>(q + r * t.ldq, r < nr ? p.n : 0);
-            s[r] = r < nr ? scale[(row + r) >> shift] : 0.f;
+            w[r] = load_codes<VEC>(q + r * t.ldq, WHOLE || r < nr ? p.n : 0);
+            s[r] = WHOLE || r < nr ? scale[(row + r) >> shift] : 0.f;
         }
     }
 };
@@ -187,17 +195,23 @@ template <typename T, bool VEC, bool E4M3>
 __global__ void __launch_bounds__(THREADS) load_kernel(Q8 in, long rows, long cols, int shift, T* y, long ldy) {
     typedef HeldCodes<VEC> Held;
     each_group<VEC, Held>(
-        rows, cols, [&](const Place& p, Held& h, long row, int nr) { h.load(in, p, row, nr, shift); },
+        rows, cols,
+        [&](const Place& p, Held& h, long row, int nr, auto whole) {
+            h.template load<decltype(whole)::value>(in, p, row, nr, shift);
+        },
         [&](const Place& p, const Held& h, long row, int nr, auto whole) {
-            constexpr bool FULL = decltype(whole)::value;
+            constexpr bool WHOLE = decltype(whole)::value;
             T* at = y + row * ldy + p.col;
 #pragma unroll
             for (int r = 0; r < RPW; ++r) {
                 float v[4];
                 decode4(h.w[r], E4M3, v);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] *= h.s[r];
-                store4<T, VEC>(at + r * ldy, FULL || r < nr ? p.n : 0, v);
+                uint64_t o[2];
+                pairs(v, o);
+                o[0] = mul2(o[0], pair(h.s[r]));
+                o[1] = mul2(o[1], pair(h.s[r]));
+                unpairs(o, v);
+                store4<T, VEC>(at + r * ldy, WHOLE || r < nr ? p.n : 0, v);
             }
         });
 }
@@ -208,13 +222,15 @@ __global__ void __launch_bounds__(THREADS)
     typedef HeldRows<T, VEC> Held;
     each_group<VEC, Held>(
         rows, cols,
-        [&](const Place& p, Held& h, long row, int nr) { h.load(z + row * ldz + p.col, ldz, p.n, nr); },
+        [&](const Place& p, Held& h, long row, int nr, auto whole) {
+            h.template load<decltype(whole)::value>(z + row * ldz + p.col, ldz, p.n, nr);
+        },
         [&](const Place& p, const Held& h, long row, int nr, auto whole) {
-            constexpr bool FULL = decltype(whole)::value;
+            constexpr bool WHOLE = decltype(whole)::value;
             float v[RPW][4];
 #pragma unroll
             for (int r = 0; r < RPW; ++r) h.x[r].values(v[r]);
-            store_rows<VEC, FULL>(z8, p, row, nr, v, E4M3);
+            store_rows<VEC, WHOLE>(z8, p, row, nr, v, E4M3);
 #pragma unroll
             for (int r = 0; r < RPW; ++r) {
                 const uint64_t o[2] = {gelu2(v[r][0], v[r][1]), gelu2(v[r][2], v[r][3])};
@@ -223,9 +239,9 @@ __global__ void __launch_bounds__(THREADS)
             if (g) {
                 T* to = g + row * ldg + p.col;
 #pragma unroll
-                for (int r = 0; r < RPW; ++r) store4<T, VEC>(to + r * ldg, FULL || r < nr ? p.n : 0, v[r]);
+                for (int r = 0; r < RPW; ++r) store4<T, VEC>(to + r * ldg, WHOLE || r < nr ? p.n : 0, v[r]);
             }
-            if (g8.q) store_rows<VEC, FULL>(g8, p, row, nr, v, g8.e4m3);
+            if (g8.q) store_rows<VEC, WHOLE>(g8, p, row, nr, v, g8.e4m3);
         });
 }
 
@@ -241,12 +257,13 @@ __global__ void __launch_bounds__(THREADS)
     typedef HeldBoth<T, VEC> Held;
     each_group<VEC, Held>(
         rows, cols,
-        [&](const Place& p, Held& h, long row, int nr) {
-            h.x.load(dg + row * lddg + p.col, lddg, p.n, nr);
-            h.c.load(z8, p, row, nr, 0);
+        [&](const Place& p, Held& h, long row, int nr, auto whole) {
+            constexpr bool WHOLE = decltype(whole)::value;
+            h.x.template load<WHOLE>(dg + row * lddg + p.col, lddg, p.n, nr);
+            h.c.template load<WHOLE>(z8, p, row, nr, 0);
         },
         [&](const Place& p, const Held& h, long row, int nr, auto whole) {
-            constexpr bool FULL = decltype(whole)::value;
+            constexpr bool WHOLE = decltype(whole)::value;
             float v[RPW][4];
 #pragma unroll
             for (int r = 0; r < RPW; ++r) {
@@ -263,9 +280,9 @@ __global__ void __launch_bounds__(THREADS)
             if (dz) {
                 T* to = dz + row * lddz + p.col;
 #pragma unroll
-                for (int r = 0; r < RPW; ++r) store4<T, VEC>(to + r * lddz, FULL || r < nr ? p.n : 0, v[r]);
+                for (int r = 0; r < RPW; ++r) store4<T, VEC>(to + r * lddz, WHOLE || r < nr ? p.n : 0, v[r]);
             }
-            if (dz8.q) store_rows<VEC, FULL>(dz8, p, row, nr, v, dz8.e4m3);
+            if (dz8.q) store_rows<VEC, WHOLE>(dz8, p, row, nr, v, dz8.e4m3);
         });
 }
 
