@@ -16,7 +16,7 @@
 // Bound by the tensor cores for large M; the adding warps need about half of the MMA's time.
 //
 // gemm_f8_small_kernel: up to 16 rows (a few tokens).  Bound by reading W once: a CTA owns 16 rows
-// of W, its warps take every fourth k-block each, and the codes go straight from global memory
+// of W, its warps take turns with the k-blocks, and the codes go straight from global memory
 // into mma.sync fragments: a lane loads 32 neighbouring codes of two rows of W and of its rows of
 // X, which is a fixed permutation of the block's k that both operands share.
 #include <cuda.h>
@@ -439,7 +439,6 @@ __global__ void __launch_bounds__(NTHREADS, 1) gemm_f8_kernel(const __grid_const
 }
 
 // ---------------------------------------------------------------------------------------
-constexpr int SM_WARPS = 4;   // k-blocks of a CTA go round its warps
 constexpr int SM_ROWS = 16;   // rows of W a CTA owns
 constexpr int SM_MAX_M = 16;
 
@@ -468,41 +467,55 @@ __device__ __forceinline__ void load32(const uint8_t* row, long k, long K, bool 
         }
 }
 
-// MT groups of eight rows of X
+// what a lane needs of a k-block: codes of two rows of W and MT rows of X, and the products of scales
 template <int MT>
-__global__ void __launch_bounds__(SM_WARPS * 32) gemm_f8_small_kernel(const uint8_t* x, long ldx, const uint8_t* w,
-                                                                      long ldw, const Params p) {
-    __shared__ float part[SM_WARPS][8 * MT][SM_ROWS + 1];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const long n0 = (long)blockIdx.x * SM_ROWS;
-    float acc[MT][4] = {};
-#pragma unroll 2
-    for (int kb = warp; kb < p.nk; kb += SM_WARPS) {
+struct SmallBlock {
+    uint32_t a[2][8], b[MT][8];
+    float s[MT][2];
+    __device__ __forceinline__ void load(const uint8_t* x, long ldx, const uint8_t* w, long ldw, const Params& p, long n,
+                                         int g, int t, int kb) {
         const long k = (long)kb * BK + 32 * t;
-        uint32_t a[2][8], b[MT][8];
-        load32(w + (n0 + g) * ldw, k, p.K, n0 + g < p.N, a[0]);
-        load32(w + (n0 + g + 8) * ldw, k, p.K, n0 + g + 8 < p.N, a[1]);
-        float s[MT][2];
-        const float sw = p.sw[(long)kb * p.ldsw + n0 / 128];
+        load32(w, k, p.K, n < p.N, a[0]);
+        load32(w + 8 * ldw, k, p.K, n + 8 < p.N, a[1]);
+        const float sw = p.sw[(long)kb * p.ldsw + n / 128];
 #pragma unroll
         for (int j = 0; j < MT; ++j) {
-            load32(x + (8 * j + g) * ldx, k, p.K, 8 * j + g < p.M, b[j]);
+            load32(x + 8 * j * ldx, k, p.K, 8 * j + g < p.M, b[j]);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const int m = 8 * j + 2 * t + c;
                 s[j][c] = m < p.M ? sw * p.sx[(long)kb * p.ldsx + m] : 0.f;
             }
         }
+    }
+};
+
+// MT groups of eight rows of X; WARPS share the k-blocks.  A warp has its next block's loads under way
+// while it multiplies: the kernel is a chain of HBM latencies otherwise.
+template <int MT, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32) gemm_f8_small_kernel(const uint8_t* x, long ldx, const uint8_t* w,
+                                                                   long ldw, const Params p) {
+    __shared__ float part[WARPS][8 * MT][SM_ROWS + 1];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const long n0 = (long)blockIdx.x * SM_ROWS, n = n0 + g;
+    x += g * ldx;
+    w += n * ldw;
+    float acc[MT][4] = {};
+    SmallBlock<MT> next;
+    if (warp < p.nk) next.load(x, ldx, w, ldw, p, n, g, t, warp);
+    for (int kb = warp; kb < p.nk; kb += WARPS) {
+        const SmallBlock<MT> now = next;
+        if (kb + WARPS < p.nk) next.load(x, ldx, w, ldw, p, n, g, t, kb + WARPS);
 #pragma unroll
         for (int j = 0; j < MT; ++j) {
             float d[4] = {};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const uint32_t f[4] = {a[0][2 * i], a[1][2 * i], a[0][2 * i + 1], a[1][2 * i + 1]};
-                mma_sync_e4m3(d, f, b[j][2 * i], b[j][2 * i + 1]);
+                const uint32_t f[4] = {now.a[0][2 * i], now.a[1][2 * i], now.a[0][2 * i + 1], now.a[1][2 * i + 1]};
+                mma_sync_e4m3(d, f, now.b[j][2 * i], now.b[j][2 * i + 1]);
             }
 #pragma unroll
-            for (int c = 0; c < 4; ++c) acc[j][c] = fmaf(d[c], s[j][c & 1], acc[j][c]);
+            for (int c = 0; c < 4; ++c) acc[j][c] = fmaf(d[c], now.s[j][c & 1], acc[j][c]);
         }
     }
 #pragma unroll
@@ -510,17 +523,22 @@ __global__ void __launch_bounds__(SM_WARPS * 32) gemm_f8_small_kernel(const uint
 #pragma unroll
         for (int c = 0; c < 4; ++c) part[warp][8 * j + 2 * t + (c & 1)][g + 8 * (c >> 1)] = acc[j][c];
     __syncthreads();
-    for (int i = threadIdx.x; i < 8 * MT * SM_ROWS; i += SM_WARPS * 32) {
+    for (int i = threadIdx.x; i < 8 * MT * SM_ROWS; i += WARPS * 32) {
         const int m = i / SM_ROWS, r = i % SM_ROWS;
-        const long n = n0 + r;
-        if (m >= p.M || n >= p.N) continue;
+        if (m >= p.M || n0 + r >= p.N) continue;
         float v = 0.f;
 #pragma unroll
-        for (int q = 0; q < SM_WARPS; ++q) v += part[q][m][r];
-        if (p.bias) v += p.bias[n];
-        const long at = m * p.ldy + n;
+        for (int q = 0; q < WARPS; ++q) v += part[q][m][r];
+        if (p.bias) v += p.bias[n0 + r];
+        const long at = m * p.ldy + n0 + r;
         put_value(p, at, p.accumulate ? old_value(p, at) + v : v);
     }
+}
+
+template <int MT, int WARPS>
+void launch_small(const GemmF8& a, const Params& p, cudaStream_t s) {
+    gemm_f8_small_kernel<MT, WARPS><<<(unsigned)((a.N + SM_ROWS - 1) / SM_ROWS), WARPS * 32, 0, s>>>(
+        a.x.q, a.x.ldq, a.w.q, a.w.ldq, p);
 }
 
 template <int BN, bool MN, bool SPLIT>
@@ -592,9 +610,9 @@ void gemm_f8(const GemmF8& a, cudaStream_t s) {
     p.mt = p.nt = p.dm = p.dn = 0;
     p.splits = 1;
     if (a.M <= SM_MAX_M && !a.w_mn) {
-        const unsigned ctas = (unsigned)((a.N + SM_ROWS - 1) / SM_ROWS);
-        if (a.M <= 8) gemm_f8_small_kernel<1><<<ctas, SM_WARPS * 32, 0, s>>>(a.x.q, a.x.ldq, a.w.q, a.w.ldq, p);
-        else gemm_f8_small_kernel<2><<<ctas, SM_WARPS * 32, 0, s>>>(a.x.q, a.x.ldq, a.w.q, a.w.ldq, p);
+        // as many warps as leave each one or two k-blocks, as far as registers let all CTAs run at once
+        if (a.M <= 8) p.nk > 16 ? launch_small<1, 16>(a, p, s) : launch_small<1, 8>(a, p, s);
+        else p.nk > 16 ? launch_small<2, 8>(a, p, s) : launch_small<2, 4>(a, p, s);
         return;
     }
     const long mt = (a.M + BM - 1) / BM, sms = current_sm_count(), narrow = mt * ((a.N + 127) / 128);
