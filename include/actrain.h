@@ -332,8 +332,8 @@ int act_lora_linear(int device, const float* x, int64_t rows, int in, int out, i
  * the legacy default stream), nothing is allocated, and every call may be captured into a CUDA
  * graph.  Tensors are row-major with a row stride in elements (ld >= columns); element types are
  * ACT_TYPE_F32, ACT_TYPE_F16 and ACT_TYPE_BF16, and base pointers are aligned to the element.
- * Any stride and alignment is taken; vectors move when bases and strides are multiples of four
- * elements.  Outputs must not overlap inputs unless said otherwise.  rows = 0 does nothing (and
+ * Any stride and alignment is taken; vectors move when bases, strides and columns are multiples
+ * of four elements.  Outputs must not overlap inputs unless said otherwise.  rows = 0 does nothing (and
  * zeroes sums over the rows that are not accumulated).  The same call gives the same bits every
  * time on the same GPU model: no reduction depends on the order in which blocks finish.
  *
@@ -397,8 +397,9 @@ int act_gelu_ckpt8_bwd(const void* dg, int dg_type, int64_t lddg, const act_ckpt
 
 /* Rank product with a checkpoint, the lora_A gradient (src/ac/lora.h:34-95) from a kept input:
  *   C[j][c] (+)= alpha * sum over rows t of U[t][j] * X[t][c],   C fp32 [nb][cols], 1 <= nb <= 64.
- * X in blocks of 1 row; its codes start on 16-byte boundaries (q and ldq multiples of 16).
- * accumulate 0 overwrites C.  status: a device int that the caller zeroes once and may read at
+ * X in blocks of 1 row, its scales powers of two as act_ckpt8_store leaves them; its codes start on
+ * 16-byte boundaries (q and ldq multiples of 16).  All of U's precision enters the product (fp32 U
+ * included) and sums are fp32; an infinite U makes its row of C NaN.  accumulate 0 overwrites C.  status: a device int that the caller zeroes once and may read at
  * any time; nonzero means that a bounded wait inside the kernel ran out and C is not valid. */
 int act_rank_gemm_ckpt8(const void* u, int u_type, int64_t ldu, int nb, const act_ckpt8* x, int64_t rows,
                         int64_t cols, float alpha, float* c, int64_t ldc, int accumulate, int32_t* status,
@@ -406,7 +407,8 @@ int act_rank_gemm_ckpt8(const void* u, int u_type, int64_t ldu, int nb, const ac
 /* Product of two E4M3 tensors, X [M][K] in blocks of one row and W in blocks of 128 rows:
  *   Y[m][n] = sum over k of X[m][k] * W[n][k] (+ bias[n]) (+ Y[m][n] with accumulate 1).
  * W is stored [N][K] (w_mn_major 0: a projection) or [K][N] (1: the input gradient dY W of a
- * weight [K = out][N = in], the same codes as the projection's).  Scales may be any fp32 values.
+ * weight [K = out][N = in], the same codes as the projection's).  Scales may be any fp32 values; a
+ * block's two are multiplied with each other first.
  * Codes start on 16-byte boundaries (q and ldq multiples of 16).  bias fp32 [N] or NULL.  Sums are
  * fp32.  status as in act_rank_gemm_ckpt8. */
 int act_gemm_f8(const act_ckpt8* x, const act_ckpt8* w, int64_t M, int64_t N, int64_t K, int w_mn_major,

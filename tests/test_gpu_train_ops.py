@@ -425,6 +425,33 @@ def test_gelu_with_checkpoint(rows, cols, kind, layout):
         assert first.shape == dz8.codes().shape
 
 
+def test_results_in_whole_numbers():
+    # the 8-bit forms of the results come as I8 too
+    rng = np.random.default_rng(12)
+    rows, cols = 20, 300
+    x = Mat(rng.standard_normal((rows, cols)), "f32")
+    y, st, y8 = out_mat(rows, cols, "f32"), Mat(np.zeros((2, rows)), "f32"), Eight(rows, cols, A.CKPT_I8)
+    A.layernorm_fwd(x.ptr, A.TYPE_F32, rows, cols, 0, 0, y.ptr, A.TYPE_F32, st.ptr, st.ptr + 4 * st.ld, y8=y8.v,
+                    stream=stream())
+    g, g8, z8, dz8 = out_mat(rows, cols, "f32"), *(Eight(rows, cols, A.CKPT_I8) for _ in range(3))
+    A.gelu_ckpt8_fwd(x.ptr, A.TYPE_F32, rows, cols, g.ptr, A.TYPE_F32, z8.v, g8=g8.v, stream=stream())
+    dz = out_mat(rows, cols, "f32")
+    A.gelu_ckpt8_bwd(g.ptr, A.TYPE_F32, z8.v, rows, cols, dz.ptr, A.TYPE_F32, dz8=dz8.v, stream=stream())
+    torch.cuda.synchronize()
+    for wide, eight in ((y, y8), (g, g8), (dz, dz8)):  # exactly the codes of the fp32 result beside them
+        q, s = E.encode(wide.np(), A.CKPT_I8)
+        np.testing.assert_array_equal(eight.codes().cpu().numpy(), q)
+        np.testing.assert_array_equal(eight.scales(), s)
+
+
+def test_gelu_of_infinities():
+    z, g, z8 = Mat(np.array([[np.inf, -np.inf, np.nan, 1e38, -1e38]]), "f32"), out_mat(1, 5, "f32"), Eight(1, 5, A.CKPT_I8)
+    A.gelu_ckpt8_fwd(z.ptr, A.TYPE_F32, 1, 5, g.ptr, A.TYPE_F32, z8.v, stream=stream())
+    torch.cuda.synchronize()
+    got = g.np()[0]
+    assert got[0] == np.inf and got[1] == 0 and np.isnan(got[2]) and got[3] == z.np()[0, 3] and got[4] == 0
+
+
 def test_gelu_over_the_whole_range():
     Z = np.concatenate([np.linspace(-14, 14, 20001), [0.0, -0.0, 60.0, -60.0, 1e30, -1e30]])[None]
     z = Mat(Z, "f32")
