@@ -45,6 +45,8 @@ constexpr int MAX_SPLIT = 8;       // portable cluster size
 constexpr int SCALE_SLOTS = 8;
 constexpr int SCALE_LD = BM + 4;  // floats
 constexpr int SCALE_BYTES = SCALE_SLOTS * SCALE_LD * 4;
+constexpr int TURN_LD = 17;  // floats of a row of 16 that a warp turns for rows of y that are not aligned
+constexpr int TURN_BYTES = 32 * TURN_LD * 4;
 
 // BN: columns of a tile
 template <int BN>
@@ -53,7 +55,8 @@ struct Shape {
     static constexpr int STAGES = BN == 256 ? 4 : 6;
     static constexpr int HALF = BN / 2;  // columns of an adding warp
     static constexpr int SCALE_OFF = STAGES * STAGE;
-    static constexpr int BAR_OFF = SCALE_OFF + SCALE_BYTES;
+    static constexpr int TURN_OFF = SCALE_OFF + SCALE_BYTES;
+    static constexpr int BAR_OFF = TURN_OFF + ADDERS * TURN_BYTES;
     static constexpr int SMEM = BAR_OFF + 8 * (2 * STAGES + 5) + 16 + 1024 /*align*/;
     static constexpr int TMEM = 2 * BN;
     static_assert(STAGES + 2 <= SCALE_SLOTS, "a scale would be overwritten before it is read");
@@ -104,29 +107,15 @@ __device__ __forceinline__ void load_sector(const void* p, uint32_t w[8]) {
                  : "memory");
 }
 
-// 16 columns n .. n + 15 of a row: bias, old value, one rounding; at counts elements of y.  Whole
-// groups of aligned rows move as 32-byte sectors (a thread's neighbours hold other rows).
+// 16 columns n .. n + 15 of an aligned row (all of them exist): bias, old value, one rounding; at
+// counts elements of y.  They move as whole 32-byte sectors (a thread's neighbours hold other rows).
 __device__ __forceinline__ void put16(const Params& p, long at, long n, float v[16]) {
-    const int left = p.N - n < 16 ? (int)(p.N - n) : 16;
-    if (left <= 0) return;
-    if (p.bias) {
-        if (left == 16 && p.vec)
+    if (p.bias)
 #pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                const float4 b = __ldg(reinterpret_cast<const float4*>(p.bias + n + i));
-                v[i] += b.x; v[i + 1] += b.y; v[i + 2] += b.z; v[i + 3] += b.w;
-            }
-        else
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (i < left) v[i] += __ldg(p.bias + n + i);
-    }
-    if (left < 16 || !p.vec) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-            if (i < left) put_value(p, at + i, p.accumulate ? old_value(p, at + i) + v[i] : v[i]);
-        return;
-    }
+        for (int i = 0; i < 16; i += 4) {
+            const float4 b = __ldg(reinterpret_cast<const float4*>(p.bias + n + i));
+            v[i] += b.x; v[i + 1] += b.y; v[i + 2] += b.z; v[i + 3] += b.w;
+        }
     if (p.y_type == OP_F32) {
         float* y = static_cast<float*>(p.y) + at;
 #pragma unroll
@@ -161,6 +150,34 @@ __device__ __forceinline__ void put16(const Params& p, long at, long n, float v[
     for (int i = 0; i < 8; ++i)
         w[i] = half ? pack_f16(v[2 * i], v[2 * i + 1]) : pack_bf16(v[2 * i], v[2 * i + 1]);
     store_sector(y, w);
+}
+
+// A lane's column n of the 32 rows from m0 on, every other row of them, from a warp's turned 16 columns:
+// bias, old value, one rounding.
+__device__ __forceinline__ void put_column(const Params& p, long m0, long n, const float* turn) {
+    const int lane = threadIdx.x & 31, first = lane >> 4;
+    const int rows = p.M - m0 < 32 ? (int)(p.M - m0) : 32;
+    const float add = p.bias ? __ldg(p.bias + n) : 0.f;
+    const float* from = turn + first * TURN_LD + (lane & 15);
+    const long at = (m0 + first) * p.ldy + n, step = 2 * p.ldy;
+    if (p.accumulate) {
+        for (int r = first; r < rows; r += 2, from += 2 * TURN_LD) {
+            const long o = at + (r - first) / 2 * step;
+            put_value(p, o, old_value(p, o) + (*from + add));
+        }
+    } else if (p.y_type == OP_F32) {
+        float* y = static_cast<float*>(p.y) + at;
+#pragma unroll 4
+        for (int r = first; r < rows; r += 2, from += 2 * TURN_LD, y += step) *y = *from + add;
+    } else {
+        uint16_t* y = static_cast<uint16_t*>(p.y) + at;
+        const bool half = p.y_type == OP_F16;
+#pragma unroll 4
+        for (int r = first; r < rows; r += 2, from += 2 * TURN_LD, y += step) {
+            const float v = *from + add;
+            *y = half ? __half_as_ushort(__float2half_rn(v)) : __bfloat16_as_ushort(__float2bfloat16_rn(v));
+        }
+    }
 }
 
 // the tiles of one CTA, column tiles first: CTAs that run together share rows of X
@@ -383,19 +400,28 @@ __global__ void __launch_bounds__(NTHREADS, 1) gemm_f8_kernel(const __grid_const
                 }
                 break;
             }
-            // epilogue: a row per thread, 16 columns at a time
+            // epilogue, 16 columns at a time: a row per thread where its pieces are whole sectors; else the
+            // warp turns its 32 rows in shared memory and writes two of them at a time
             const long m = m0 + lane;
-            if (m < p.M) {
+            float* turn = reinterpret_cast<float*>(smem + S::TURN_OFF + (warp - 4) * TURN_BYTES);
 #pragma unroll
-                for (int c = 0; c < S::HALF / 16; ++c) {
-                    float v[16];
+            for (int c = 0; c < S::HALF / 16; ++c) {
+                const long n = n0 + 16 * c;
+                float v[16];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float2 f = unpair(acc[8 * c + i]);
-                        v[2 * i] = f.x;
-                        v[2 * i + 1] = f.y;
-                    }
-                    put16(p, m * p.ldy + n0 + 16 * c, n0 + 16 * c, v);
+                for (int i = 0; i < 8; ++i) {
+                    const float2 f = unpair(acc[8 * c + i]);
+                    v[2 * i] = f.x;
+                    v[2 * i + 1] = f.y;
+                }
+                if (p.vec && n + 16 <= p.N) {
+                    if (m < p.M) put16(p, m * p.ldy + n, n, v);
+                } else if (n < p.N) {
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) turn[lane * TURN_LD + i] = v[i];
+                    __syncwarp();
+                    if (n + (lane & 15) < p.N) put_column(p, m0, n + (lane & 15), turn);
                 }
             }
         }
@@ -490,8 +516,8 @@ struct SmallBlock {
     }
 };
 
-// MT groups of eight rows of X; WARPS share the k-blocks.  A warp has its next block's loads under way
-// while it multiplies: the kernel is a chain of HBM latencies otherwise.
+// MT groups of eight rows of X; WARPS share the k-blocks.  A warp has more than one block's loads under
+// way: the kernel is a chain of HBM latencies otherwise.
 template <int MT, int WARPS>
 __global__ void __launch_bounds__(WARPS * 32) gemm_f8_small_kernel(const uint8_t* x, long ldx, const uint8_t* w,
                                                                    long ldw, const Params p) {
@@ -501,11 +527,7 @@ __global__ void __launch_bounds__(WARPS * 32) gemm_f8_small_kernel(const uint8_t
     x += g * ldx;
     w += n * ldw;
     float acc[MT][4] = {};
-    SmallBlock<MT> next;
-    if (warp < p.nk) next.load(x, ldx, w, ldw, p, n, g, t, warp);
-    for (int kb = warp; kb < p.nk; kb += WARPS) {
-        const SmallBlock<MT> now = next;
-        if (kb + WARPS < p.nk) next.load(x, ldx, w, ldw, p, n, g, t, kb + WARPS);
+    auto multiply = [&](const SmallBlock<MT>& now) {
 #pragma unroll
         for (int j = 0; j < MT; ++j) {
             float d[4] = {};
@@ -516,6 +538,22 @@ __global__ void __launch_bounds__(WARPS * 32) gemm_f8_small_kernel(const uint8_t
             }
 #pragma unroll
             for (int c = 0; c < 4; ++c) acc[j][c] = fmaf(d[c], now.s[j][c & 1], acc[j][c]);
+        }
+    };
+    if (MT == 1) {
+        SmallBlock<MT> next;
+        if (warp < p.nk) next.load(x, ldx, w, ldw, p, n, g, t, warp);
+        for (int kb = warp; kb < p.nk; kb += WARPS) {
+            const SmallBlock<MT> now = next;
+            if (kb + WARPS < p.nk) next.load(x, ldx, w, ldw, p, n, g, t, kb + WARPS);
+            multiply(now);
+        }
+    } else {  // two blocks at a time: a third would cost the registers that let all CTAs run at once
+#pragma unroll 2
+        for (int kb = warp; kb < p.nk; kb += WARPS) {
+            SmallBlock<MT> now;
+            now.load(x, ldx, w, ldw, p, n, g, t, kb);
+            multiply(now);
         }
     }
 #pragma unroll
