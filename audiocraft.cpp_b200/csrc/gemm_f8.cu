@@ -432,6 +432,9 @@ __global__ void __launch_bounds__(NTHREADS, 1) gemm_f8_kernel(const __grid_const
     if (warp == 0)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::TMEM));
     if (SPLIT) {
+        // every warp has the launch's registers again for what all of them do from here on
+        if (warp < 4) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+        else asm volatile("setmaxnreg.dec.sync.aligned.u32 168;");
         // every thread of every CTA of the cluster passes both barriers
         cluster_sync_all();
         const Walk<SPLIT> w(p);

@@ -393,6 +393,9 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    // every warp has the launch's registers again for what all of them do from here on
+    if (warp < 4) asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 128;");
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (warp == 0)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::TMEM));
