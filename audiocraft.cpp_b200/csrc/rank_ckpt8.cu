@@ -15,6 +15,7 @@
 //              accumulators are emptied into fp32 registers every 256 rows (two in turn where they fit)
 // The slices of a column tile form a cluster and add their sums in order through distributed
 // shared memory: no atomics, the same bits every time.
+// 24000 x 6144, rank 64: 104 us with fp32 U (1.5 TB/s; shared memory and conversion take over from HBM).
 #include <cuda.h>
 
 #include <atomic>
@@ -39,7 +40,7 @@ constexpr int RROWS = RK / RCONV;        // rows of a block each takes
 constexpr int RTHREADS = (8 + RCONV) * 32;
 constexpr int RA_BYTES = 128 * RK * 2;   // bf16 operand of 128 columns
 constexpr int RB_BOX = RK * 64 * 2;      // 64 columns of pieces
-constexpr int RMAX_SPLIT = 8;            // portable cluster size
+constexpr int RMAX_SPLIT = 16;           // cluster size, beyond the portable 8 by opt-in
 
 // T: tiles of 128 columns per CTA; P: pieces of U
 template <int T, int P>
@@ -446,13 +447,14 @@ void launch(const RankCkpt8& a, RParams p, cudaStream_t s) {
         cudaFuncSetAttribute(rank_kernel<T, E4M3, U>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
     });
     const long tiles = (a.cols + T * 128 - 1) / (T * 128);
-    // slices per tile: the least rounds of clusters times blocks of a slice
+    // slices per tile: the least rounds of clusters times the blocks of a slice and what a round costs
+    // besides (start, join), about as long as eight blocks
     p.splits = 1;
     static std::atomic<int> known[RMAX_SPLIT + 1][64];
     long best = -1;
     for (int n = 1; n <= RMAX_SPLIT && n <= p.nk; ++n) {
         const long at_once = clusters_at_once(rank_kernel<T, E4M3, U>, RTHREADS, S::SMEM, n, known[n]);
-        const long cost = (tiles + at_once - 1) / at_once * ((p.nk + n - 1) / n);
+        const long cost = (tiles + at_once - 1) / at_once * ((p.nk + n - 1) / n + 8);
         if (best < 0 || cost < best) {
             best = cost;
             p.splits = n;
@@ -499,7 +501,7 @@ void rank_ckpt8(const RankCkpt8& a, cudaStream_t s) {
     p.splits = 1; p.status = a.status;
     // 256 columns a CTA halve the work on U per code, where that still leaves CTAs for most SMs
     const long wide = (a.cols + 255) / 256;
-    if (wide * RMAX_SPLIT >= current_sm_count()) a.x.e4m3 ? launch<2, true>(a, p, s) : launch<2, false>(a, p, s);
+    if (wide * 8 >= current_sm_count()) a.x.e4m3 ? launch<2, true>(a, p, s) : launch<2, false>(a, p, s);
     else a.x.e4m3 ? launch<1, true>(a, p, s) : launch<1, false>(a, p, s);
 }
 
