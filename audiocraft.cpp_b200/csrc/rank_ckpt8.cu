@@ -5,6 +5,8 @@
 // codes into tensor-core operands keeps up.  A CTA owns 128 or 256 columns of X (the rows of the MMA)
 // and a slice of the rows t (the reduction), in blocks of 64:
 //   warp 0     TMA: raw codes into a ring of 64-row blocks
+//   warps 2, 3 U and the scales into the same ring (cp.async; loads to the converting warps' registers one
+//              block ahead came too late: 24000 x 6144, rank 16, f16 U 94 us, so 70)
 //   warps 8-15 codes * scale -> bf16 (exact: 4 or 7 significant bits times a power of two) in the
 //              128-byte-swizzled MN-major layout; the block's rows of U, cut into bf16 pieces that add
 //              up to it exactly (one for bf16, two for f16, three for fp32): both operands of the
@@ -15,11 +17,11 @@
 //              accumulators are emptied into fp32 registers every 256 rows (two in turn where they fit)
 // The slices of a column tile form a cluster and add their sums in order through distributed
 // shared memory: no atomics, the same bits every time.
-// 24000 x 6144, rank 64: 104 us with fp32 U (1.5 TB/s; shared memory and conversion take over from HBM).
+// 24000 x 6144: rank 16 with f16 U 70 us (2.2 TB/s), rank 64 with bf16 U 90 us, with fp32 U 109 us
+// (shared memory and conversion take over from HBM).
 #include <cuda.h>
 
 #include <atomic>
-#include <climits>
 #include <cstring>
 #include <type_traits>
 
@@ -41,22 +43,30 @@ constexpr int RTHREADS = (8 + RCONV) * 32;
 constexpr int RA_BYTES = 128 * RK * 2;   // bf16 operand of 128 columns
 constexpr int RB_BOX = RK * 64 * 2;      // 64 columns of pieces
 constexpr int RMAX_SPLIT = 16;           // cluster size, beyond the portable 8 by opt-in
+constexpr int RNU = (RROWS * 8 + 31) / 32;  // units of 8 columns of U that a lane converts
+constexpr int RSMEM_MAX = 232448;
 
-// T: tiles of 128 columns per CTA; P: pieces of U
-template <int T, int P>
+// T: tiles of 128 columns per CTA; P: pieces of U, E: bytes of one of its values
+template <int T, int P, int E>
 struct RShape {
     static constexpr int RAW = T * 128 * RK;
-    static constexpr int RAWS = T == 2 ? 6 : 8;
     static constexpr int OP = T * RA_BYTES + P * RB_BOX;
     static constexpr int OPS = T == 2 ? 2 : 3;
     static constexpr int ACC = P * 64;                      // TMEM columns of a tile's accumulator
     static constexpr int BUFS = 2 * T * ACC <= 512 ? 2 : 1;  // of all tiles' accumulators
     static constexpr int TMEM = BUFS * T * ACC <= 128 ? 128 : BUFS * T * ACC <= 256 ? 256 : 512;
+    static constexpr int U_BYTES = RCONV * 32 * RNU * 8 * E;  // U of a block
+    static constexpr int SC_BYTES = T * RK * 4;               // its scales
     static constexpr int RAW_OFF = OPS * OP;
-    static constexpr int BAR_OFF = RAW_OFF + RAWS * RAW;
+    static constexpr int FIT = (RSMEM_MAX - 2048 - RAW_OFF) / (RAW + U_BYTES + SC_BYTES);
+    static constexpr int RAWS = FIT < 8 ? FIT : 8;
+    static constexpr int U_OFF = RAW_OFF + RAWS * RAW;
+    static constexpr int SC_OFF = U_OFF + RAWS * U_BYTES;
+    static constexpr int BAR_OFF = SC_OFF + RAWS * SC_BYTES;
     static constexpr int NBARS = 2 * RAWS + 2 * OPS + 5;
     static constexpr int SMEM = BAR_OFF + 8 * NBARS + 16 + 1024 /*align*/;
     static constexpr int LD = T * 128 + 4;   // floats of a row of the sums in shared memory
+    static_assert(RAWS >= 3 && SMEM <= RSMEM_MAX, "shared memory");
     static_assert(64 * LD * 4 <= RAW_OFF, "the sums take the operand ring's place");
 };
 
@@ -64,7 +74,7 @@ struct RParams {
     int rows, nk, nb, nbp;  // nbp: nb rounded up to 16
     long cols;
     const void* u;
-    int u_vec;
+    int u_copy;  // bytes of a copy of U to shared memory: 16 or 8; 0: through registers
     long ldu;
     const float* scale;
     long lds;
@@ -78,6 +88,17 @@ struct RParams {
 struct RMaps {
     CUtensorMap x;
 };
+
+// B bytes, or zeros when !is (nothing is read then)
+template <int B>
+__device__ __forceinline__ void cp_async_to(uint32_t to, const void* from, bool is) {
+    if (B == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(is ? 16 : 0)
+                     : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(from), "n"(B), "r"(is ? B : 0)
+                     : "memory");
+}
 
 __device__ __forceinline__ uint32_t pair_bf16(uint64_t v) {
     const float2 f = unpair(v);
@@ -119,26 +140,27 @@ __device__ __forceinline__ uint4 codes_to_bf16(uint2 w, float s) {
     return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
-// Eight neighbouring values of a row of U as they lie in memory: as words where base, stride and
-// nb allow, else one by one; `have` counts the columns from the first one (0: none), missing
-// ones are 0.
+// Eight neighbouring values of a row of U as they lie in memory; `have` counts the columns from the
+// first one (0: none), missing ones are 0.
 template <typename U>
 struct UnitOfU {
-    static constexpr int WORDS = 8 * sizeof(U) / 8;  // 8-byte words
-    uint2 w[WORDS];
-    __device__ __forceinline__ void load(const U* at, int have, bool vec) {
-#pragma unroll
-        for (int i = 0; i < WORDS; ++i) w[i] = make_uint2(0, 0);
-        if (vec) {
-            if (have > 0)  // nb is a multiple of eight here: all or nothing
-#pragma unroll
-                for (int i = 0; i < WORDS; ++i) w[i] = reinterpret_cast<const uint2*>(at)[i];
-            return;
-        }
+    static constexpr int W16 = 8 * sizeof(U) / 16;  // 16-byte words
+    uint4 w[W16];
+    __device__ __forceinline__ void load(const U* at, int have) {
         U e[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) e[i] = i < have ? at[i] : U(0.f);
         memcpy(w, e, sizeof(e));
+    }
+    // from global to shared memory in pieces of B bytes; word i of the unit lies at to + 512 i
+    template <int B>
+    static __device__ __forceinline__ void copy(uint32_t to, const U* at, int have) {
+#pragma unroll
+        for (int i = 0; i < 128 / B * (int)sizeof(U) / 16; ++i) {
+            constexpr int V = B / (int)sizeof(U);
+            const bool is = i * V < have;
+            cp_async_to<B>(to + i * B / 16 * 512 + i * B % 16, at + (is ? i * V : 0), is);
+        }
     }
     __device__ __forceinline__ void values(float v[8]) const {
         U e[8];
@@ -157,7 +179,7 @@ struct Pieces {
 template <int T, bool E4M3, typename U>
 __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant__ RMaps maps, const RParams p) {
     constexpr int PIECES = Pieces<U>::N;
-    typedef RShape<T, PIECES> S;
+    typedef RShape<T, PIECES, sizeof(U)> S;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t base = (raw + 1023) & ~1023u;
@@ -179,7 +201,7 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
     if (threadIdx.x == 0) {
         prefetch_tmap(&maps.x);
         for (int s = 0; s < S::RAWS; ++s) {
-            mbar_init(raw_full(s), 1);
+            mbar_init(raw_full(s), 1 + 64);  // and every lane of warps 2 and 3
             mbar_init(raw_empty(s), RCONV);
         }
         for (int s = 0; s < S::OPS; ++s) {
@@ -259,6 +281,48 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
                 mma_commit(drained);
                 mbar_drain_inline(drained, 0);
             }
+        } else if (warp >= 2) {
+            // -------------------------------------------------------- U and scales
+            // Copied as they are, each unit to where the lane that converts it reads it.
+            constexpr int W16 = UnitOfU<U>::W16;
+            const int w0 = (warp - 2) * (RCONV / 2);  // for converting warps w0 .. w0 + RCONV / 2 - 1
+            const int units = p.nbp >> 3;
+            int s = 0;
+            uint32_t ph = 0;
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (!__all_sync(FULL_WARP, mbar_wait_inline(raw_empty(s), ph ^ 1, p.status, 48))) break;
+                const int t0 = kb * RK;
+#pragma unroll
+                for (int j = 0; j < T; ++j) {
+                    const int e = ((warp - 2) * T + j) * 32 + lane, r = e % RK;
+                    const long cb = c0 / BLOCK + e / RK;
+                    const bool is = cb * BLOCK < p.cols && t0 + r < p.rows;
+                    cp_async_to<4>(base + S::SC_OFF + s * S::SC_BYTES + 4 * e,
+                                   is ? p.scale + cb * p.lds + t0 + r : p.scale, is);
+                }
+#pragma unroll
+                for (int i = 0; i < RNU; ++i) {
+                    const int q = lane + 32 * i, uj = q % units, ur = q / units;
+                    if (ur >= RROWS || !p.u_copy) break;
+                    const int have = p.nb - 8 * uj;
+                    uint32_t to = base + S::U_OFF + s * S::U_BYTES + (w0 * RNU + i) * W16 * 512 + 16 * lane;
+                    int t = t0 + w0 * RROWS + ur;
+                    const U* at = static_cast<const U*>(p.u) + (long)t * p.ldu + 8 * uj;
+#pragma unroll 1
+                    for (int c = 0; c < RCONV / 2; ++c) {
+                        const int n = t < p.rows && have > 0 ? have : 0;
+                        const U* a = n ? at : static_cast<const U*>(p.u);
+                        if (p.u_copy == 16) UnitOfU<U>::template copy<16>(to, a, n);
+                        else UnitOfU<U>::template copy<8>(to, a, n);
+                        t += RROWS;
+                        at += RROWS * p.ldu;
+                        to += RNU * W16 * 512;
+                    }
+                }
+                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(raw_full(s)) : "memory");
+                if (++s == S::RAWS) { s = 0; ph ^= 1; }
+            }
+            cp_async_wait_all();
         }
     } else if (warp < 8) {
         // ------------------------------------------------------------ sums
@@ -311,9 +375,10 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
         const int cw = warp - 8, r0 = RROWS * cw;  // rows r0 .. r0 + RROWS - 1 of each block
         const int cl = lane % LPR, tile = cl >> 4, box = (cl >> 3) & 1, unit = cl & 7;
         // U: RROWS x nbp / 8 units of 8 columns, up to NU a lane
-        constexpr int NU = (RROWS * 8 + 31) / 32;
+        constexpr int NU = RNU;
         const int units = p.nbp >> 3;
-        int ur[NU], have[NU];  // a unit's row in the warp's part and its columns that exist (0: no unit)
+        bool has[NU];
+        int ur[NU], have[NU];  // a unit's row in the warp's part and its columns that exist
         const U* from[NU];
         // where its pieces go in an operand slot: piece after piece, end to end
         uint32_t u_to[NU][PIECES];
@@ -321,7 +386,8 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
         for (int i = 0; i < NU; ++i) {
             const int q = lane + 32 * i, uj = q % units;
             ur[i] = q / units;
-            have[i] = ur[i] < RROWS ? p.nb - 8 * uj : INT_MIN;
+            has[i] = ur[i] < RROWS;
+            have[i] = has[i] ? p.nb - 8 * uj : 0;
             from[i] = static_cast<const U*>(p.u) + (long)(r0 + ur[i]) * p.ldu + 8 * uj;
 #pragma unroll
             for (int piece = 0; piece < PIECES; ++piece) {
@@ -329,32 +395,37 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
                 u_to[i][piece] = T * RA_BYTES + (col8 >> 3) * RB_BOX + q8_sw128(r0 + ur[i], col8 & 7);
             }
         }
-        const long fb = c0 / BLOCK + lane / RROWS;  // whose scale lanes 0 .. RROWS T - 1 fetch
-        const bool fetch = lane < RROWS * T && fb * BLOCK < p.cols;
-        const float* scales = p.scale + (fetch ? fb * p.lds : 0) + lane % RROWS;
+        // Values at odd places are loaded by their own lane one block ahead: copies of 4 bytes keep warps 2
+        // and 3 longer (22317 x 25, fp32, rank 51: 37 us against 27).
         UnitOfU<U> un[NU];
-        float sn = 0.f;
-        auto prefetch = [&](int kb) {
-            const int t0 = kb * RK + r0;
+        auto load = [&](int kb) {
 #pragma unroll
             for (int i = 0; i < NU; ++i)
-                un[i].load(from[i] + (long)kb * RK * p.ldu, t0 + ur[i] < p.rows ? have[i] : 0, p.u_vec);
-            sn = fetch && t0 + lane % RROWS < p.rows ? scales[t0] : 0.f;
+                un[i].load(from[i] + (long)kb * RK * p.ldu, kb * RK + r0 + ur[i] < p.rows ? have[i] : 0);
         };
-        if (kb0 < kb1) prefetch(kb0);
+        if (!p.u_copy && kb0 < kb1) load(kb0);
         int s = 0, o = 0;
         uint32_t ph = 0, oph = 0;
         for (int kb = kb0; kb < kb1; ++kb) {
             float u[NU][8];
-            const float sc = sn;
+            if (!p.u_copy) {
 #pragma unroll
-            for (int i = 0; i < NU; ++i) un[i].values(u[i]);
-            if (kb + 1 < kb1) prefetch(kb + 1);
+                for (int i = 0; i < NU; ++i) un[i].values(u[i]);
+                if (kb + 1 < kb1) load(kb + 1);
+            }
             // every lane waits (a lane that waited for its warp would cost the warp a detour); they agree
             const bool got = mbar_wait_inline(op_empty(o), oph ^ 1, p.status, 46) &&
                              mbar_wait_inline(raw_full(s), ph, p.status, 47);
             if (!__all_sync(FULL_WARP, got)) break;
             unsigned char* op = smem + o * S::OP;
+            if (p.u_copy)
+#pragma unroll
+                for (int i = 0; i < NU; ++i)
+#pragma unroll
+                    for (int j = 0; j < UnitOfU<U>::W16; ++j)
+                        un[i].w[j] = *reinterpret_cast<const uint4*>(
+                            smem + S::U_OFF + s * S::U_BYTES + ((cw * NU + i) * UnitOfU<U>::W16 + j) * 512 + 16 * lane);
+            const float* sc = reinterpret_cast<const float*>(smem + S::SC_OFF + s * S::SC_BYTES) + tile * RK + r0;
             const unsigned char* rw = smem + S::RAW_OFF + s * S::RAW;
             uint2 w[RROWS / RPP];
 #pragma unroll
@@ -363,16 +434,19 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
 #pragma unroll
             for (int i = 0; i < RROWS / RPP; ++i) {
                 const int r = i * RPP + lane / LPR;
-                const float sr = __shfl_sync(FULL_WARP, sc, RROWS * tile + r);
                 *reinterpret_cast<uint4*>(op + tile * RA_BYTES + box * 8192 + q8_sw128(r0 + r, unit)) =
-                    codes_to_bf16<E4M3>(w[i], sr);
+                    codes_to_bf16<E4M3>(w[i], sc[r]);
             }
-            if (lane == 0) mbar_arrive(raw_empty(s));  // after the shuffles: every lane has read its codes
+            if (p.u_copy)
+#pragma unroll
+                for (int i = 0; i < NU; ++i) un[i].values(u[i]);
+            __syncwarp();  // every lane has read the slot
+            if (lane == 0) mbar_arrive(raw_empty(s));
             // The next piece of a value is its upper half-word (cut off, not rounded: three pieces hold all
             // 24 bits and none can overflow); what is left of it is exact.
 #pragma unroll
             for (int i = 0; i < NU; ++i) {
-                if (have[i] == INT_MIN) break;
+                if (!has[i]) break;
 #pragma unroll
                 for (int piece = 0; piece < PIECES; ++piece) {
                     uint32_t h[4];
@@ -441,7 +515,7 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
 
 template <int T, bool E4M3, typename U>
 void launch(const RankCkpt8& a, RParams p, cudaStream_t s) {
-    typedef RShape<T, Pieces<U>::N> S;
+    typedef RShape<T, Pieces<U>::N, sizeof(U)> S;
     static DeviceOnce once;
     once([] {
         cudaFuncSetAttribute(rank_kernel<T, E4M3, U>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
@@ -495,7 +569,11 @@ void rank_ckpt8(const RankCkpt8& a, cudaStream_t s) {
     p.rows = (int)a.rows; p.nk = (int)((a.rows + RK - 1) / RK); p.nb = a.nb; p.nbp = (a.nb + 15) / 16 * 16;
     p.cols = a.cols;
     p.u = a.u.p; p.ldu = a.u.ld;
-    p.u_vec = a.nb % 8 == 0 && a.u.ld * op_bytes(a.u.type) % 8 == 0 && reinterpret_cast<uintptr_t>(a.u.p) % 8 == 0;
+    // the widest copy that base, stride and row length allow
+    const int eb = op_bytes(a.u.type);
+    p.u_copy = 0;
+    for (int b = 16; b >= 8 && !p.u_copy; b >>= 1)
+        if (a.nb * eb % b == 0 && a.u.ld * eb % b == 0 && reinterpret_cast<uintptr_t>(a.u.p) % b == 0) p.u_copy = b;
     p.scale = a.x.scale; p.lds = a.x.lds; p.alpha = a.alpha;
     p.c = a.c; p.ldc = a.ldc; p.c_vec = vec4(a.c) && a.ldc % 4 == 0 ? 1 : 0; p.accumulate = a.accumulate ? 1 : 0;
     p.splits = 1; p.status = a.status;

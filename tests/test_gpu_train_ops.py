@@ -522,6 +522,26 @@ def test_rank_product(rows, cols, nb, kind, ut):
         assert c.untouched() and st.item() == 0
 
 
+@pytest.mark.parametrize("rows,cols,nb,pad,off", [(200, 4737, 8, 4, 4), (200, 4737, 24, 8, 8), (65, 4992, 64, 0, 0),
+                                                  (513, 130, 40, 4, 12), (1, 4800, 16, 8, 4), (63, 5001, 19, 1, 2)])
+@pytest.mark.parametrize("kind", [A.CKPT_I8, A.CKPT_E4M3], ids=["i8", "e4m3"])
+@pytest.mark.parametrize("ut", ALL)
+def test_rank_product_of_wide_inputs_and_placed_u(rows, cols, nb, pad, off, kind, ut):
+    """256 columns a CTA, and U at 16-byte, 8-byte and odd places."""
+    rng = np.random.default_rng(rows + cols + nb + pad + off)
+    q, s = E.encode(wild(rng, rows, cols), kind)
+    x = Eight(rows, cols, kind, 1, up16(cols), 0, data=(q, s))
+    u, c, st = Mat(rng.standard_normal((rows, nb)), ut, pad, off), out_mat(nb, cols, "f32"), status_word()
+    for _ in range(2):
+        A.rank_gemm_ckpt8(u.ptr, E.KINDS[ut], nb, x.v, rows, cols, c.ptr, st.data_ptr(), ldu=u.ld, ldc=c.ld,
+                          stream=stream())
+    torch.cuda.synchronize()
+    K, V = E.decode(q, s, kind), u.np()
+    # rows terms in any order, twice that for truncating adds
+    assert_close(c.np(), V.T @ K, (2 * rows + 4) * U * (np.abs(V).T @ np.abs(K)) + 2.0 ** -140, "c")
+    assert c.untouched() and st.item() == 0
+
+
 def test_rank_product_of_no_rows():
     c = Mat(np.ones((4, 40)), "f32", 3)
     x, st = Eight(1, 40, A.CKPT_I8, 1, 8), status_word()
