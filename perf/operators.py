@@ -24,18 +24,8 @@ FORMATS = {"i8": (127.0, 7, 127.0 / 128.0), "e4m3": (448.0, 9, 0.875)}  # top = 
 EPS = 1e-5
 
 
-_binding = None
-
-
 def _lib():
-    """The framework's binding, imported once; its folder is no package name, so it goes on the path."""
-    global _binding
-    if _binding is None:
-        _binding = _import()
-    return _binding
-
-
-def _import():
+    """The framework's binding; its folder is no package name, so it goes on the path."""
     here = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "audiocraft.cpp_b200")
     if here not in sys.path:
         sys.path.insert(0, here)
