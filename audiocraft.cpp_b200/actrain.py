@@ -21,6 +21,7 @@ FAMILY_MELODYFLOW, FAMILY_MUSICGEN = 0, 1
 ADAPTER_LORA, ADAPTER_DORA_ROWS = 0, 1
 TYPE_F32, TYPE_F16, TYPE_Q8_0, TYPE_BF16 = 0, 1, 8, 30
 CKPT_I8, CKPT_E4M3 = 1, 2
+COPY_PROBE_BYTES, COPY_PROBE_CODE = 8192, 98
 TARGETS = ("self.qkv", "self.out", "cross.q", "cross.kv", "cross.out", "ff.0", "ff.2")
 # kernel families counted by act_path_counts (ACT_PATH_*)
 PATHS = ("attn_fwd_tc", "attn_fwd_mma", "attn_bwd_tc", "attn_bwd_mma", "gemm_tc", "gemm_mma", "rank_tc",
@@ -141,6 +142,7 @@ SIGNATURES = {
                                       C.c_float, C.c_void_p, C.c_int64, C.c_int, C.c_void_p, C.c_void_p]),
     "act_gemm_f8": (C.c_int, [C.POINTER(Ckpt8), C.POINTER(Ckpt8)] + [C.c_int64] * 3 + [C.c_int, C.c_void_p, C.c_void_p,
                               C.c_int, C.c_int64, C.c_int, C.c_void_p, C.c_void_p]),
+    "act_copy_wait_probe": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p]),
     "act_rank_gemm_f16": (C.c_int, [C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int,
                                      C.c_int, C.c_int, C.c_float, C.c_int, C.c_int, C.POINTER(C.c_float)]),
     "act_rank_gemm_q8_0": (C.c_int, [C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int,
@@ -598,6 +600,13 @@ def gemm_f8(x8, w8, M, N, K, y, y_type, status, w_mn_major=False, bias=0, accumu
     """act_gemm_f8: Y [M][N] (+)= X8 W8^T (+ bias), W8 [N][K] or, with w_mn_major, [K][N]."""
     rc = (_lib or lib()).act_gemm_f8(x8, w8, M, N, K, int(w_mn_major), bias, y, y_type, ldy or N, int(accumulate),
                                      status, stream)
+    if rc:
+        _failed(rc)
+
+
+def copy_wait_probe(src, dst, limit_ns, status, stream=0):
+    """act_copy_wait_probe: COPY_PROBE_BYTES from src to dst, around a wait that runs out after limit_ns."""
+    rc = (_lib or lib()).act_copy_wait_probe(src, dst, limit_ns, status, stream)
     if rc:
         _failed(rc)
 

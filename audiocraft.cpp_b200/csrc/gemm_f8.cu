@@ -278,11 +278,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) gemm_f8_kernel(const __grid_const
                     if (++s == S::STAGES) { s = 0; ph ^= 1; }
                 }
             }
-            if (!ok)  // let what was issued land before the CTA ends
-                for (long j = 0; j < S::STAGES && j < issued; ++j) {
-                    const long i = issued - 1 - j;
-                    mbar_drain_inline(full_bar((int)(i % S::STAGES)), (uint32_t)((i / S::STAGES) & 1));
-                }
+            drain_ring(full_bar(0), S::STAGES, issued);
         } else if (warp == 2) {
             // -------------------------------------------------------- scales
             int s = 0, slot = 0;
@@ -349,10 +345,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) gemm_f8_kernel(const __grid_const
                     if (b == 0) bph ^= 1;
                 }
             }
-            if (!ok) {  // the MMAs in flight write TMEM: wait for them before it is freed
-                mma_commit(drained);
-                mbar_drain_inline(drained, 0);
-            }
+            drain_mma(drained);
         }
     } else {
         // ------------------------------------------------------------ adding warps

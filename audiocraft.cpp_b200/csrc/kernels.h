@@ -302,6 +302,10 @@ void adamw(float* value, float* m, float* v, float* grad, const uint8_t* decay_m
 // limit_ns nanoseconds with WAIT_PROBE_CODE recorded in *err (wait_probe.cu).
 constexpr int WAIT_PROBE_CODE = 99;
 void wait_probe(const int* flag, long long limit_ns, int* err, cudaStream_t s);
+// COPY_PROBE_BYTES from src to dst through shared memory, between the two a bounded wait on a barrier
+// that nobody arrives on: COPY_PROBE_CODE in *status after limit_ns nanoseconds.
+constexpr int COPY_PROBE_CODE = 98, COPY_PROBE_BYTES = 8192;
+void copy_wait_probe(const void* src, void* dst, long long limit_ns, int* status, cudaStream_t s);
 
 // Q8_0 blocks -> f16 (one-time weight binding) and fp32 (parity checks).
 void q8_0_to_f16(const uint8_t* blocks, long nblocks, f16* out, cudaStream_t s);

@@ -233,18 +233,13 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
             // -------------------------------------------------------- TMA
             int s = 0, issued = 0;
             uint32_t ph = 0;
-            bool ok = true;
             for (int kb = kb0; kb < kb1; ++kb, ++issued) {
-                if (!mbar_wait_inline(raw_empty(s), ph ^ 1, p.status, 41)) { ok = false; break; }
+                if (!mbar_wait_inline(raw_empty(s), ph ^ 1, p.status, 41)) break;
                 mbar_expect_tx(raw_full(s), S::RAW);
                 tma_load_2d(base + S::RAW_OFF + s * S::RAW, &maps.x, (int)c0, kb * RK, raw_full(s));
                 if (++s == S::RAWS) { s = 0; ph ^= 1; }
             }
-            if (!ok)  // let what was issued land before the CTA ends
-                for (int j = 0; j < S::RAWS && j < issued; ++j) {
-                    const int i = issued - 1 - j;
-                    mbar_drain_inline(raw_full(i % S::RAWS), (uint32_t)((i / S::RAWS) & 1));
-                }
+            drain_ring(raw_full(0), S::RAWS, issued);
         } else if (warp == 1 && lane == 0) {
             // -------------------------------------------------------- MMA
             // fp32 accumulator, bf16 operands (1), both MN-major, N >> 3, M >> 4
@@ -255,11 +250,10 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
             constexpr uint32_t step = 2048 >> 4;  // 16 rows of 128 bytes
             int s = 0, b = 0;
             uint32_t ph = 0, bph = 0;
-            bool ok = true;
             for (int kb = kb0; kb < kb1; ++kb) {
                 const int in_group = (kb - kb0) % RGROUP;
-                if (in_group == 0 && !mbar_wait_inline(acc_empty(b), bph ^ 1, p.status, 42)) { ok = false; break; }
-                if (!mbar_wait_inline(op_full(s), ph, p.status, 43)) { ok = false; break; }
+                if (in_group == 0 && !mbar_wait_inline(acc_empty(b), bph ^ 1, p.status, 42)) break;
+                if (!mbar_wait_inline(op_full(s), ph, p.status, 43)) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint64_t off = (uint64_t)((s * S::OP) >> 4);
 #pragma unroll
@@ -277,10 +271,7 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
                     if (++b == S::BUFS) { b = 0; bph ^= 1; }
                 }
             }
-            if (!ok) {  // the MMAs in flight write TMEM: wait for them before it is freed
-                mma_commit(drained);
-                mbar_drain_inline(drained, 0);
-            }
+            drain_mma(drained);
         } else if (warp >= 2) {
             // -------------------------------------------------------- U and scales
             // Copied as they are, each unit to where the lane that converts it reads it.

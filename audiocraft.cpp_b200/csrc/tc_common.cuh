@@ -73,11 +73,12 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int* er
 
 // The same wait without a call, for code whose warps took registers from others (setmaxnreg): a call
 // would have to save them all.
-__device__ __forceinline__ bool mbar_wait_inline(uint32_t bar, uint32_t parity, int* err, int code) {
+__device__ __forceinline__ bool mbar_wait_inline(uint32_t bar, uint32_t parity, int* err, int code,
+                                                 unsigned long long limit_ns = WAIT_NS) {
     if (mbar_try(bar, parity)) return true;
     const unsigned long long t0 = globaltimer();
     while (!mbar_try_sleep(bar, parity, 100000u)) {
-        if (globaltimer() - t0 > WAIT_NS) {
+        if (globaltimer() - t0 > limit_ns) {
             atomicCAS(err, 0, code);
             return false;
         }
@@ -89,6 +90,17 @@ __device__ __forceinline__ void mbar_drain_inline(uint32_t bar, uint32_t parity)
     const unsigned long long t0 = globaltimer();
     while (!mbar_try_sleep(bar, parity, 20000u))
         if (globaltimer() - t0 > 100000000ull) return;
+}
+
+// The end of a role that filled a ring of `stages` slots with asynchronous copies, `issued` fills in
+// all, each completing a phase of its slot's barrier (full + 8 * slot): no copy may land after the
+// CTA has left its shared memory.  Whether its own waits held or not: a role that has issued
+// everything cannot know whether the one that consumes gave up.
+__device__ __forceinline__ void drain_ring(uint32_t full, int stages, long issued) {
+    for (long j = 0; j < stages && j < issued; ++j) {
+        const long i = issued - 1 - j;
+        mbar_drain_inline(full + 8 * (uint32_t)(i % stages), (uint32_t)((i / stages) & 1));
+    }
 }
 
 // Wait for copies this thread issued to land before its CTA exits, after another wait failed:
@@ -216,6 +228,13 @@ __device__ __forceinline__ void mma_f8(uint32_t tmem_d, uint64_t adesc, uint64_t
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
                  : "memory");
+}
+
+// The end of a role that issued MMAs: they write TMEM and read shared memory, so they are done before
+// either is given up, also when the role that reads their sums has given up.  bar: used by nothing else.
+__device__ __forceinline__ void drain_mma(uint32_t bar) {
+    mma_commit(bar);
+    mbar_drain_inline(bar, 0);
 }
 
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {

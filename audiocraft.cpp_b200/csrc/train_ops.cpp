@@ -345,6 +345,20 @@ extern "C" int act_rank_gemm_ckpt8(const void* u, int u_type, int64_t ldu, int n
     });
 }
 
+extern "C" int act_copy_wait_probe(const void* src, void* dst, int64_t limit_ns, int32_t* status, void* stream) {
+    return guarded("act_copy_wait_probe", [&](Checker& c) {
+        c.size(limit_ns, 1, 10000000000ll, "limit_ns");
+        c.raw(src, 16, "src");
+        c.raw(dst, 1, "dst");
+        c.raw(status, 4, "status");
+        c.where(src, "src");
+        c.where(dst, "dst");
+        c.where(status, "status");
+        act::copy_wait_probe(src, dst, limit_ns, status, on(stream));
+        c.done();
+    });
+}
+
 extern "C" int act_gemm_f8(const act_ckpt8* x, const act_ckpt8* w, int64_t M, int64_t N, int64_t K, int w_mn_major,
                            const float* bias, void* y, int y_type, int64_t ldy, int accumulate, int32_t* status,
                            void* stream) {

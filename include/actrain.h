@@ -414,6 +414,14 @@ int act_rank_gemm_ckpt8(const void* u, int u_type, int64_t ldu, int nb, const ac
 int act_gemm_f8(const act_ckpt8* x, const act_ckpt8* w, int64_t M, int64_t N, int64_t K, int w_mn_major,
                 const float* bias, void* y, int y_type, int64_t ldy, int accumulate, int32_t* status, void* stream);
 
+/* Failure-path check of both products' status word: one kernel copies ACT_COPY_PROBE_BYTES from src to
+ * dst through shared memory; between the two it waits, as the products do, for something that never
+ * comes, gives up after limit_ns (1 ns .. 10 s), writes ACT_COPY_PROBE_CODE to *status (if that is 0)
+ * and waits for its copies in flight as they do.  src 16-byte aligned; all three are device pointers. */
+#define ACT_COPY_PROBE_BYTES 8192
+#define ACT_COPY_PROBE_CODE 98
+int act_copy_wait_probe(const void* src, void* dst, int64_t limit_ns, int32_t* status, void* stream);
+
 #if defined(__GNUC__)
 #pragma GCC visibility pop
 #endif

@@ -37,3 +37,13 @@ def test_waits_order_memory_for_the_compiler(name):
     for s in statements(text):
         if any(w in s for w in WAITS):
             assert "volatile" in s and '"memory"' in s, " ".join(s.split())
+
+
+@pytest.mark.parametrize("name", ["gemm_f8.cu", "rank_ckpt8.cu"])
+def test_products_drain_their_copies_and_mmas_on_every_path(name):
+    # a role whose own waits all held still has copies or MMAs in flight if the role after it gave up
+    text = open(os.path.join(CSRC, name)).read()
+    for call in ("drain_ring(", "drain_mma("):
+        at = text.index(call)
+        before = text[:at].rstrip()
+        assert before.endswith("}") and text.count(call) == 1, "not the unconditional end of its role's loop"
