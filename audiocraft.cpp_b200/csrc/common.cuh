@@ -51,13 +51,14 @@ inline int current_sm_count() {
 }
 
 // How many clusters of `size` CTAs of a kernel run at once on the current device: the GPU's
-// processing clusters differ in size, so this is not the SM count over the size.  `known` is the
-// caller's own cache for this kernel and size, one entry per device ordinal.
+// processing clusters differ in size, so this is not the SM count over the size.  0: none does (a part of
+// a GPU may have no processing cluster that large).  `known` is the caller's own cache for this
+// kernel and size, one entry per device ordinal: 0 not asked yet, -1 none.
 template <typename Kernel>
 inline int clusters_at_once(Kernel* kern, int threads, size_t smem, int size, std::atomic<int> (&known)[64]) {
     int dev = 0, n = 0;
     const bool cached = cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64;
-    if (cached && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
+    if (cached && (n = known[dev].load(std::memory_order_relaxed)) != 0) return n > 0 ? n : 0;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)size, 1, 1);
     cfg.blockDim = dim3((unsigned)threads, 1, 1);
@@ -73,7 +74,8 @@ inline int clusters_at_once(Kernel* kern, int threads, size_t smem, int size, st
         (size > 8 && cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) ||
         cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n < 1) {
         cudaGetLastError();
-        return 1;
+        if (cached) known[dev].store(-1, std::memory_order_relaxed);
+        return 0;
     }
     if (cached) known[dev].store(n, std::memory_order_relaxed);
     return n;

@@ -26,6 +26,7 @@
 #include <atomic>
 
 #include "ckpt8.cuh"
+#include "slices.h"
 #include "tc_common.cuh"
 
 namespace act {
@@ -620,22 +621,14 @@ void launch(const GemmF8& a, const Params& p, cudaStream_t s) {
     else launch<BN, false, SPLIT>(a, p, s);
 }
 
-// CTAs per tile for a product of few tiles: the least rounds of clusters times the k-blocks of a
-// slice and what joining the slices costs, about as long as twelve k-blocks
+// CTAs per tile for a product of tiles that all run at once: joining the slices costs about as long as
+// twelve k-blocks
 template <bool MN>
 int best_split(long tiles, int nk) {
     static std::atomic<int> known[MAX_SPLIT + 1][64];
-    int splits = 1;
-    long best = nk;
-    for (int n = 2; n <= MAX_SPLIT && n <= nk; ++n) {
-        const long at_once = clusters_at_once(gemm_f8_kernel<128, MN, true>, NTHREADS, Shape<128>::SMEM, n, known[n]);
-        const long cost = (tiles + at_once - 1) / at_once * ((nk + n - 1) / n + 12);
-        if (cost < best) {
-            best = cost;
-            splits = n;
-        }
-    }
-    return splits;
+    return best_slices(tiles, nk, MAX_SPLIT, 12, nk, [](int n) {
+        return clusters_at_once(gemm_f8_kernel<128, MN, true>, NTHREADS, Shape<128>::SMEM, n, known[n]);
+    });
 }
 
 }  // namespace

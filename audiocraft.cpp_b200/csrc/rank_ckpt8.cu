@@ -26,6 +26,7 @@
 #include <type_traits>
 
 #include "ckpt8.cuh"
+#include "slices.h"
 #include "tc_common.cuh"
 
 namespace act {
@@ -512,19 +513,12 @@ void launch(const RankCkpt8& a, RParams p, cudaStream_t s) {
         cudaFuncSetAttribute(rank_kernel<T, E4M3, U>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
     });
     const long tiles = (a.cols + T * 128 - 1) / (T * 128);
-    // slices per tile: the least rounds of clusters times the blocks of a slice and what a round costs
-    // besides (start, join), about as long as eight blocks
-    p.splits = 1;
+    // slices per tile: a round costs about eight blocks besides its own (start, join), without slices too
     static std::atomic<int> known[RMAX_SPLIT + 1][64];
-    long best = -1;
-    for (int n = 1; n <= RMAX_SPLIT && n <= p.nk; ++n) {
-        const long at_once = clusters_at_once(rank_kernel<T, E4M3, U>, RTHREADS, S::SMEM, n, known[n]);
-        const long cost = (tiles + at_once - 1) / at_once * ((p.nk + n - 1) / n + 8);
-        if (best < 0 || cost < best) {
-            best = cost;
-            p.splits = n;
-        }
-    }
+    auto at_once = [](int n) { return clusters_at_once(rank_kernel<T, E4M3, U>, RTHREADS, S::SMEM, n, known[n]); };
+    constexpr int JOIN = 8;
+    const long room = at_once(1) > 1 ? at_once(1) : 1;
+    p.splits = best_slices(tiles, p.nk, RMAX_SPLIT, JOIN, (tiles + room - 1) / room * (p.nk + JOIN), at_once);
     RMaps maps;
     tc_make_map_raw(&maps.x, a.x.q, false, a.rows, a.cols, a.x.ldq, T * 128, RK);
     cudaLaunchConfig_t cfg = {};
