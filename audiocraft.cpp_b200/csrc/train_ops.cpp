@@ -57,7 +57,9 @@ struct Checker {
             refuse(name + ": " + what + " is on device " + std::to_string(at.device) + ", the current device is " +
                    std::to_string(device));
     }
-    void raw(const void* p, size_t align, const char* what) const {
+    // rows: of the tensor; one without any may be NULL, as the address of an empty tensor is
+    void raw(const void* p, size_t align, const char* what, int64_t rows = 1) const {
+        if (!p && rows == 0) return;
         if (!p) refuse(name + ": " + what + " is NULL");
         if (reinterpret_cast<uintptr_t>(p) % align)
             refuse(name + ": " + what + " must be " + std::to_string(align) + "-byte aligned");
@@ -68,10 +70,10 @@ struct Checker {
         if (ggml == ACT_TYPE_BF16) return act::OP_BF16;
         refuse(name + ": " + what + " type " + std::to_string(ggml) + " (ACT_TYPE_F32, _F16 or _BF16)");
     }
-    OpTensor tensor(const void* p, int ggml, int64_t ld, int64_t cols, const char* what) const {
+    OpTensor tensor(const void* p, int ggml, int64_t ld, int64_t rows, int64_t cols, const char* what) const {
         OpTensor t;
         t.type = type(ggml, what);
-        raw(p, act::op_bytes(t.type), what);
+        raw(p, act::op_bytes(t.type), what, rows);
         if (ld < cols || ld > kMaxSize)
             refuse(name + ": row stride of " + what + " is " + std::to_string(ld) + " for " + std::to_string(cols) +
                    " columns");
@@ -84,8 +86,8 @@ struct Checker {
         if (!v) refuse(name + ": " + what + " is NULL");
         if (v->type != ACT_CKPT_I8 && v->type != ACT_CKPT_E4M3)
             refuse(name + ": " + what + " has type " + std::to_string(v->type) + " (ACT_CKPT_I8 or _E4M3)");
-        raw(v->q, pitch, what);
-        raw(v->scale, 4, (std::string(what) + "'s scale").c_str());
+        raw(v->q, pitch, what, rows);
+        raw(v->scale, 4, (std::string(what) + "'s scale").c_str(), rows);
         if (v->ldq < cols || v->ldq > kMaxSize || v->ldq % pitch)
             refuse(name + ": row stride of " + what + " is " + std::to_string(v->ldq) + " for " +
                    std::to_string(cols) + " columns (a multiple of " + std::to_string(pitch) + ")");
@@ -154,7 +156,7 @@ extern "C" int act_ckpt8_store(const void* x, int x_type, int64_t ldx, int64_t r
         c.size(rows, 0, kMaxSize - 1, "rows");
         c.size(cols, 1, kMaxSize - 1, "cols");
         block(c, block_rows);
-        const OpTensor tx = c.tensor(x, x_type, ldx, cols, "x");
+        const OpTensor tx = c.tensor(x, x_type, ldx, rows, cols, "x");
         const Q8 t = c.codes(out, rows, cols, block_rows, 1, "out");
         if (!rows) return;
         c.where(tx, "x");
@@ -170,7 +172,7 @@ extern "C" int act_ckpt8_load(const act_ckpt8* in, int64_t rows, int64_t cols, i
         c.size(rows, 0, kMaxSize - 1, "rows");
         c.size(cols, 1, kMaxSize - 1, "cols");
         block(c, block_rows);
-        const OpTensor ty = c.tensor(y, y_type, ldy, cols, "y");
+        const OpTensor ty = c.tensor(y, y_type, ldy, rows, cols, "y");
         const Q8 t = c.codes(in, rows, cols, block_rows, 1, "in");
         if (!rows) return;
         c.where(t, "in");
@@ -187,16 +189,16 @@ extern "C" int act_layernorm_fwd(const void* x, int x_type, int64_t ldx, int64_t
         c.size(rows, 0, kMaxSize - 1, "rows");
         c.size(dim, 1, act::LN_MAX_DIM, "dim");
         if (!(eps >= 0.f) || std::isinf(eps)) refuse(c.name + ": eps must be finite and not negative");
-        if (!y && !y8) refuse(c.name + ": y and y8 are both NULL");
+        if (rows && !y && !y8) refuse(c.name + ": y and y8 are both NULL");
         act::LnFwd a;
-        a.x = c.tensor(x, x_type, ldx, dim, "x");
-        if (y) a.y = c.tensor(y, y_type, ldy, dim, "y");
+        a.x = c.tensor(x, x_type, ldx, rows, dim, "x");
+        if (y) a.y = c.tensor(y, y_type, ldy, rows, dim, "y");
         if (y8) a.y8 = c.codes(y8, rows, dim, 1, 1, "y8");
         if (x8) a.x8 = c.codes(x8, rows, dim, 1, 1, "x8");
         if (w) c.raw(w, 4, "w");
         if (b) c.raw(b, 4, "b");
-        c.raw(mean, 4, "mean");
-        c.raw(rstd, 4, "rstd");
+        c.raw(mean, 4, "mean", rows);
+        c.raw(rstd, 4, "rstd", rows);
         if (!rows) return;
         c.where(a.x, "x");
         c.where(a.y, "y");
@@ -231,16 +233,16 @@ extern "C" int act_layernorm_bwd(const void* dy, int dy_type, int64_t lddy, cons
         c.size(rows, 0, kMaxSize - 1, "rows");
         c.size(dim, 1, act::LN_MAX_DIM, "dim");
         c.flag(accumulate, "accumulate");
-        if (!x == !x8) refuse(c.name + ": exactly one of x and x8 must be given");
+        if (x ? x8 != nullptr : !x8 && rows) refuse(c.name + ": exactly one of x and x8 must be given");
         act::LnBwd a;
-        a.dy = c.tensor(dy, dy_type, lddy, dim, "dy");
-        if (x) a.x = c.tensor(x, x_type, ldx, dim, "x");
+        a.dy = c.tensor(dy, dy_type, lddy, rows, dim, "dy");
+        if (x) a.x = c.tensor(x, x_type, ldx, rows, dim, "x");
         if (x8) a.x8 = c.codes(x8, rows, dim, 1, 1, "x8");
-        a.dx = c.tensor(dx, dx_type, lddx, dim, "dx");
-        if (add) a.add = c.tensor(add, dx_type, lddx, dim, "add");
+        a.dx = c.tensor(dx, dx_type, lddx, rows, dim, "dx");
+        if (add) a.add = c.tensor(add, dx_type, lddx, rows, dim, "add");
         if (w) c.raw(w, 4, "w");
-        c.raw(mean, 4, "mean");
-        c.raw(rstd, 4, "rstd");
+        c.raw(mean, 4, "mean", rows);
+        c.raw(rstd, 4, "rstd", rows);
         if (dw) c.raw(dw, 4, "dw");
         if (db) c.raw(db, 4, "db");
         c.raw(workspace, 16, "workspace");
@@ -278,11 +280,11 @@ extern "C" int act_gelu_ckpt8_fwd(const void* z, int z_type, int64_t ldz, int64_
     return guarded("act_gelu_ckpt8_fwd", [&](Checker& c) {
         c.size(rows, 0, kMaxSize - 1, "rows");
         c.size(cols, 1, kMaxSize - 1, "cols");
-        if (!g && !g8) refuse(c.name + ": g and g8 are both NULL");
-        const OpTensor tz = c.tensor(z, z_type, ldz, cols, "z");
+        if (rows && !g && !g8) refuse(c.name + ": g and g8 are both NULL");
+        const OpTensor tz = c.tensor(z, z_type, ldz, rows, cols, "z");
         OpTensor tg;
         Q8 t8;
-        if (g) tg = c.tensor(g, z_type, ldg, cols, "g");
+        if (g) tg = c.tensor(g, z_type, ldg, rows, cols, "g");
         if (g8) t8 = c.codes(g8, rows, cols, 1, 1, "g8");
         const Q8 tk = c.codes(z8, rows, cols, 1, 1, "z8");
         if (!rows) return;
@@ -300,12 +302,12 @@ extern "C" int act_gelu_ckpt8_bwd(const void* dg, int dg_type, int64_t lddg, con
     return guarded("act_gelu_ckpt8_bwd", [&](Checker& c) {
         c.size(rows, 0, kMaxSize - 1, "rows");
         c.size(cols, 1, kMaxSize - 1, "cols");
-        if (!dz && !dz8) refuse(c.name + ": dz and dz8 are both NULL");
-        const OpTensor tg = c.tensor(dg, dg_type, lddg, cols, "dg");
+        if (rows && !dz && !dz8) refuse(c.name + ": dz and dz8 are both NULL");
+        const OpTensor tg = c.tensor(dg, dg_type, lddg, rows, cols, "dg");
         const Q8 tk = c.codes(z8, rows, cols, 1, 1, "z8");
         OpTensor tz;
         Q8 t8;
-        if (dz) tz = c.tensor(dz, dg_type, lddz, cols, "dz");
+        if (dz) tz = c.tensor(dz, dg_type, lddz, rows, cols, "dz");
         if (dz8) t8 = c.codes(dz8, rows, cols, 1, 1, "dz8");
         if (!rows) return;
         c.where(tg, "dg");
@@ -326,9 +328,9 @@ extern "C" int act_rank_gemm_ckpt8(const void* u, int u_type, int64_t ldu, int n
         c.size(nb, 1, 64, "nb");
         c.flag(accumulate, "accumulate");
         act::RankCkpt8 a;
-        a.u = c.tensor(u, u_type, ldu, nb, "u");
+        a.u = c.tensor(u, u_type, ldu, rows, nb, "u");
         a.x = c.codes(x, rows, cols, 1, 16, "x");
-        c.tensor(cp, ACT_TYPE_F32, ldc, cols, "c");
+        c.tensor(cp, ACT_TYPE_F32, ldc, nb, cols, "c");
         c.raw(status, 4, "status");
         if (!rows && accumulate) return;
         if (rows) {
@@ -373,7 +375,7 @@ extern "C" int act_gemm_f8(const act_ckpt8* x, const act_ckpt8* w, int64_t M, in
         a.w = w_mn_major ? c.codes(w, K, N, 128, 16, "w") : c.codes(w, N, K, 128, 16, "w");
         if (!a.x.e4m3 || !a.w.e4m3) refuse(c.name + ": x and w must be ACT_CKPT_E4M3");
         if (bias) c.raw(bias, 4, "bias");
-        a.y = c.tensor(y, y_type, ldy, N, "y");
+        a.y = c.tensor(y, y_type, ldy, M, N, "y");
         c.raw(status, 4, "status");
         if (!M) return;
         c.where(a.x, "x");

@@ -334,8 +334,9 @@ int act_lora_linear(int device, const float* x, int64_t rows, int in, int out, i
  * ACT_TYPE_F32, ACT_TYPE_F16 and ACT_TYPE_BF16, and base pointers are aligned to the element.
  * Any stride and alignment is taken; vectors move when bases, strides and columns are multiples
  * of four elements.  Outputs must not overlap inputs unless said otherwise.  rows = 0 does nothing (and
- * zeroes sums over the rows that are not accumulated).  The same call gives the same bits every
- * time on the same GPU model: no reduction depends on the order in which blocks finish.
+ * zeroes sums over the rows that are not accumulated); tensors with that many rows, codes and scales
+ * among them, may then be NULL, as the address of an empty tensor often is.  The same call gives the same
+ * bits every time on the same GPU model: no reduction depends on the order in which blocks finish.
  *
  * An 8-bit tensor is codes and scales.  A block is 128 neighbouring columns (the last one of a
  * row may be shorter) of one row, or of 128 rows for a weight, and has one fp32 scale: the
