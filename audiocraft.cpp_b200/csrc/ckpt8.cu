@@ -84,7 +84,7 @@ __device__ __forceinline__ void store_rows(const Q8& t, const Place& p, long row
         top[r] = __reduce_max_sync(FULL_WARP, largest(v[r]));
         most = max(most, top[r]);
     }
-    const bool bad = most >= 0x7f800000u;  // one test for all rows: something is not finite
+    const bool bad = most > ordinary(e4m3);  // one test for all rows
     if (bad)
 #pragma unroll
         for (int r = 0; r < RPW; ++r) top[r] = __reduce_max_sync(FULL_WARP, largest_finite(v[r]));
@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(THREADS) store_square_kernel(const T* x, long 
             held[r].values(v);
             any = max(any, largest(v));
         }
-        const bool bad = __syncthreads_or(any >= 0x7f800000u);
+        const bool bad = __syncthreads_or(any > ordinary(E4M3));
         if (bad) {
 #pragma unroll
             for (int r = 0; r < SQUARE_ROWS; ++r) {

@@ -88,8 +88,9 @@ __global__ void __launch_bounds__(W * G * 32) ln_fwd_kernel(const FwdParams p) {
             p.rstd[row] = rstd;
         }
         if (KEEP) {
-            // a value that is not finite makes the sum of squares so: one test a row
-            const bool bad = !(sq < __int_as_float(0x7f800000));
+            // a value that is not finite, or beyond 2^127, makes the sum of squares infinite or NaN unless it is
+            // close to the mean: one test a row
+            const bool bad = !(sq < __int_as_float(0x7f800000) && fabsf(mean) < 0x1p126f);
             uint32_t scale = 0;
 #pragma unroll
             for (int k = 0; k < NCH; ++k) {

@@ -56,3 +56,72 @@ def test_infinite_u_gives_what_the_formula_gives(rows, cols, nb, ut, kind):
         # rows terms in any order, twice that for truncating adds; the product with alpha
         assert_close(got[finite], want[finite], (2 * rows + 4) * U * size + 2.0 ** -140, "c")
         assert st.item() == 0
+
+
+def nearest_kept(x, kind, block=1):
+    """Codes and scales of the definition, and what they stand for; a value that rounds to 2^128, which fp32
+    does not have, takes the code below."""
+    q, s = E.encode(x, kind, block)
+    v = E.decode(q, s, kind, block)
+    past = np.abs(v) >= 2.0 ** 128
+    signed = q.view(np.int8).astype(np.int64)
+    if kind == A.CKPT_I8:
+        signed = np.where(past, signed - np.sign(signed), signed)
+        q = (signed & 255).astype(np.uint8)
+    else:
+        q = np.where(past, q - 1, q).astype(np.uint8)  # sign and size: one less is one step towards 0
+    return q, s, E.decode(q, s, kind, block)
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("kind", [A.CKPT_I8, A.CKPT_E4M3], ids=["i8", "e4m3"])
+@pytest.mark.parametrize("layout", [(0, 0), (3, 1)], ids=["dense", "odd"])
+def test_the_largest_finite_values_stay_finite(t, kind, layout):
+    # a mask of the type's lowest value in an activation: its checkpoint is finite, and so are the gradients
+    rng = np.random.default_rng(3)
+    pad, off = layout
+    big = torch.finfo(torch.float32 if t == "f32" else torch.bfloat16).max
+    X = rng.standard_normal((9, 300))
+    X[0, :40], X[1, 40:90], X[2, ::3], X[3, 7] = big, -big, -big, 0.99 * big
+    X[4, :], X[5, :4], X[6, 130] = -big, [big, np.inf, np.nan, -big], 0.8 * big
+    X[7, 200:204] = 0.9375 * 2.0 ** 128, 0.96875 * 2.0 ** 128, 0.984375 * 2.0 ** 128, 0.9921875 * 2.0 ** 128
+    z = Mat(X, t, pad, off)
+    for block in (1, 128):
+        e, y = Eight(9, 300, kind, block, pad, off), out_mat(9, 300, "f32", pad, off)
+        A.ckpt8_store(z.ptr, E.KINDS[t], 9, 300, e.v, block_rows=block, ldx=z.ld, stream=stream())
+        A.ckpt8_load(e.v, 9, 300, y.ptr, A.TYPE_F32, block_rows=block, ldy=y.ld, stream=stream())
+        torch.cuda.synchronize()
+        q, s, v = nearest_kept(z.np(), kind, block)
+        np.testing.assert_array_equal(e.codes().cpu().numpy(), q)
+        np.testing.assert_array_equal(e.scales(), s)
+        np.testing.assert_array_equal(y.np(), v)
+        assert np.array_equal(np.isfinite(y.np()), np.isfinite(z.np()))
+    q, s, v = nearest_kept(z.np(), kind)
+    # the norm's checkpoint of the same rows, and of rows of one column (whose variance is 0)
+    st, x8, y8 = Mat(np.zeros((2, 9)), "f32"), Eight(9, 300, kind, 1, pad, off), out_mat(9, 300, "f32")
+    A.layernorm_fwd(z.ptr, E.KINDS[t], 9, 300, 0, 0, y8.ptr, A.TYPE_F32, st.ptr, st.ptr + 4 * st.ld, ldx=z.ld, x8=x8.v,
+                    stream=stream())
+    torch.cuda.synchronize()
+    np.testing.assert_array_equal(x8.codes().cpu().numpy(), q)
+    np.testing.assert_array_equal(x8.scales(), s)
+    one = Mat(np.array([[big], [-big], [0.5], [0.9 * big]]), t)
+    st, x8, y = Mat(np.zeros((2, 4)), "f32"), Eight(4, 1, kind), out_mat(4, 1, "f32")
+    A.layernorm_fwd(one.ptr, E.KINDS[t], 4, 1, 0, 0, y.ptr, A.TYPE_F32, st.ptr, st.ptr + 4 * st.ld, x8=x8.v,
+                    stream=stream())
+    torch.cuda.synchronize()
+    np.testing.assert_array_equal(x8.np(), nearest_kept(one.np(), kind)[2])
+    # GELU there and back: its own 8-bit result too; the gradient at the kept values is 1 or 0 out there
+    z8, g8, g, dz = Eight(9, 300, kind, 1, pad, off), Eight(9, 300, kind, 1, pad, off), out_mat(9, 300, "f32"), \
+        out_mat(9, 300, t, pad, off)
+    ones = Mat(np.ones((9, 300)), t, pad, off)
+    A.gelu_ckpt8_fwd(z.ptr, E.KINDS[t], 9, 300, 0, E.KINDS[t], z8.v, g8=g8.v, ldz=z.ld, stream=stream())
+    A.ckpt8_load(g8.v, 9, 300, g.ptr, A.TYPE_F32, stream=stream())
+    A.gelu_ckpt8_bwd(ones.ptr, E.KINDS[t], z8.v, 9, 300, dz.ptr, E.KINDS[t], lddg=ones.ld, lddz=dz.ld, stream=stream())
+    torch.cuda.synchronize()
+    np.testing.assert_array_equal(z8.codes().cpu().numpy(), q)
+    far = np.abs(z.np()) > 1e30
+    right = np.isfinite(z.np())
+    np.testing.assert_array_equal(dz.np()[far & right], (z.np() > 0)[far & right].astype(float))
+    np.testing.assert_array_equal(np.isfinite(dz.np()), np.isfinite(v))
+    up = far & right & (z.np() > 0)
+    assert np.all(np.isfinite(g.np()[up])) and np.all(np.abs(g.np()[up] / z.np()[up] - 1) <= 2.0 ** -4)
