@@ -308,10 +308,10 @@ __device__ __forceinline__ uint32_t store_block(uint8_t* p, int n, const float v
 // ---------------------------------------------------------------------------------------
 // Normal distribution: Q = 1 - Phi(|z|) = P(t) exp(-z^2 / 2), t = 1 / (1 + 0.3 |z|), where P is
 // the polynomial of degree 8 fitted (iteratively reweighted least squares, relative error
-// 5.8e-8 for |z| <= 14.5, where Q leaves fp32's range) to exp(z^2 / 2) (1 - Phi(|z|)).  The form
-// keeps relative accuracy in the tail, where 1 - erf would cancel.  With the hardware's
-// reciprocal and exponential (which flushes below 2^-126) the results are within about 1e-6 of
-// gelu and gelu'.  Two values at a time: these passes are bound by issued instructions.
+// 6.8e-8 for |z| <= 14.5, where Q leaves fp32's range; evaluated in fp32 5.6e-7 with a reciprocal
+// one step off) to exp(z^2 / 2) (1 - Phi(|z|)).  The form keeps relative accuracy in the tail,
+// where 1 - erf would cancel.  With the hardware's exponential (2^-22; it flushes below 2^-126) and
+// its argument's roundings (6.7e-8 z^2) the tail is within 2^-20 + 6.7e-8 z^2 of the true one.  Two values at a time: these passes are bound by issued instructions.
 __device__ __forceinline__ float ex2(float v) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
