@@ -84,14 +84,20 @@ __device__ __forceinline__ void store_rows(const Q8& t, const Place& p, long row
         top[r] = __reduce_max_sync(FULL_WARP, largest(v[r]));
         most = max(most, top[r]);
     }
-    const bool bad = most > ordinary(e4m3);  // one test for all rows
-    if (bad)
+    if (most > limit_bits(e4m3)) {  // one test for all rows: something is beyond the limit or not finite
 #pragma unroll
-        for (int r = 0; r < RPW; ++r) top[r] = __reduce_max_sync(FULL_WARP, largest_finite(v[r]));
+        for (int r = 0; r < RPW; ++r) {
+            float w[4] = {v[r][0], v[r][1], v[r][2], v[r][3]};
+            limit4(w, e4m3);
+            s[r] = scale_bits(__reduce_max_sync(FULL_WARP, largest_finite(w)), e4m3);
+            store_codes<VEC>(q + r * t.ldq, WHOLE || r < nr ? p.n : 0, encode4(w, inverse_pow2(s[r]), e4m3, true));
+        }
+    } else {
 #pragma unroll
-    for (int r = 0; r < RPW; ++r) {
-        s[r] = scale_bits(top[r], e4m3);
-        store_codes<VEC>(q + r * t.ldq, WHOLE || r < nr ? p.n : 0, encode4(v[r], inverse_pow2(s[r]), e4m3, bad));
+        for (int r = 0; r < RPW; ++r) {
+            s[r] = scale_bits(top[r], e4m3);
+            store_codes<VEC>(q + r * t.ldq, WHOLE || r < nr ? p.n : 0, encode4(v[r], inverse_pow2(s[r]), e4m3, false));
+        }
     }
     store_scales(t, p.chunk, row, nr, s);
 }
@@ -145,12 +151,13 @@ __global__ void __launch_bounds__(THREADS) store_square_kernel(const T* x, long 
             held[r].values(v);
             any = max(any, largest(v));
         }
-        const bool bad = __syncthreads_or(any > ordinary(E4M3));
+        const bool bad = __syncthreads_or(any > limit_bits(E4M3));
         if (bad) {
 #pragma unroll
             for (int r = 0; r < SQUARE_ROWS; ++r) {
                 float v[4];
                 held[r].values(v);
+                limit4(v, E4M3);
                 m = max(m, largest_finite(v));
             }
         } else {
@@ -164,11 +171,21 @@ __global__ void __launch_bounds__(THREADS) store_square_kernel(const T* x, long 
         const uint32_t s = scale_bits(m, E4M3);
         const float inv = inverse_pow2(s);
         uint8_t* q = out.q + r0 * out.ldq + c0;
+        if (bad) {
 #pragma unroll
-        for (int r = 0; r < SQUARE_ROWS; ++r) {
-            float v[4];
-            held[r].values(v);
-            store_codes<VEC>(q + r * out.ldq, r < nr ? n : 0, encode4(v, inv, E4M3, bad));
+            for (int r = 0; r < SQUARE_ROWS; ++r) {
+                float v[4];
+                held[r].values(v);
+                limit4(v, E4M3);
+                store_codes<VEC>(q + r * out.ldq, r < nr ? n : 0, encode4(v, inv, E4M3, true));
+            }
+        } else {
+#pragma unroll
+            for (int r = 0; r < SQUARE_ROWS; ++r) {
+                float v[4];
+                held[r].values(v);
+                store_codes<VEC>(q + r * out.ldq, r < nr ? n : 0, encode4(v, inv, E4M3, false));
+            }
         }
         if (threadIdx.x == 0) out.scale[(long)blockIdx.x * out.lds + rb] = __uint_as_float(s);
         __syncthreads();  // top is read before the next block's is written

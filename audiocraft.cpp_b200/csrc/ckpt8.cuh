@@ -187,12 +187,22 @@ __device__ __forceinline__ float inverse_pow2(uint32_t s_bits) { return __uint_a
 
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
-// The largest finite |x| of a block as float bits, and whether the block is out of the ordinary (which is
-// rare and costs its own pass): it holds infinities or NaN, or a value so large that its code may
-// stand for 2^128, which fp32 does not have.  That can be with the largest scale only, so beyond top
-// times half of it: 448 * 2^119, 127 * 2^121.  Non-negative floats order like their bits, and
+// The largest value a code and a scale stand for in fp32, 240 * 2^120 or 127 * 2^121, as float bits: the
+// next code stands for 2^128.  Values beyond it are stored as it.
+__device__ __forceinline__ constexpr uint32_t limit_bits(bool e4m3) { return e4m3 ? 0x7f700000u : 0x7f7e0000u; }
+__device__ __forceinline__ float limited(float v, bool e4m3) {  // infinities and NaN stay
+    return abs_bits(v) > limit_bits(e4m3) && abs_bits(v) < 0x7f800000u
+               ? copysignf(__uint_as_float(limit_bits(e4m3)), v)
+               : v;
+}
+__device__ __forceinline__ void limit4(float v[4], bool e4m3) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = limited(v[i], e4m3);
+}
+
+// The largest finite |x| of a block as float bits, and whether the block holds anything beyond the limit or
+// not finite (which is rare and costs its own pass).  Non-negative floats order like their bits, and
 // bits >= 0x7f800000 are infinities and NaN.
-__device__ __forceinline__ constexpr uint32_t ordinary(bool e4m3) { return e4m3 ? 0x7f600000u : 0x7f7e0000u; }
 struct Top {
     uint32_t bits;
     bool bad;
@@ -211,16 +221,19 @@ __device__ __forceinline__ uint32_t largest_finite(const float v[4]) {
     for (int i = 0; i < 4; ++i) m = max(m, abs_bits(v[i]) < 0x7f800000u ? abs_bits(v[i]) : 0u);
     return m;
 }
-__device__ __forceinline__ Top warp_top(const float v[4], bool e4m3) {
+__device__ __forceinline__ Top warp_top(float v[4], bool e4m3) {  // and limits the values
     Top t;
     t.bits = __reduce_max_sync(FULL_WARP, largest(v));
-    t.bad = t.bits > ordinary(e4m3);
-    if (t.bad) t.bits = __reduce_max_sync(FULL_WARP, largest_finite(v));
+    t.bad = t.bits > limit_bits(e4m3);
+    if (t.bad) {
+        limit4(v, e4m3);
+        t.bits = __reduce_max_sync(FULL_WARP, largest_finite(v));
+    }
     return t;
 }
 
-// Four values times 1 / s (exact) -> four codes; with `bad` (a block out of the ordinary), what is not
-// finite becomes NaN, and what would round to 2^128 takes the code below (240 * 2^120, 63 * 2^122).
+// Four values within the limit times 1 / s (exact) -> four codes; with `bad`, what is not finite becomes NaN
+// first.
 // I8: adding 1.5 * 2^23 rounds to nearest even and leaves the whole number in the low byte.
 __device__ __forceinline__ uint32_t encode4(const float v[4], float inv, bool e4m3, bool bad) {
     const uint64_t i2 = pair(inv);
@@ -230,10 +243,8 @@ __device__ __forceinline__ uint32_t encode4(const float v[4], float inv, bool e4
         unpairs(m, x);
         if (bad)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (inv == 0x1p-120f) x[i] = fminf(fmaxf(x[i], -240.f), 240.f);
+            for (int i = 0; i < 4; ++i)
                 if (abs_bits(v[i]) >= 0x7f800000u) x[i] = __int_as_float(0x7fc00000);
-            }
         const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[0], x[1]), __NV_SATFINITE, __NV_E4M3);
         const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[2], x[3]), __NV_SATFINITE, __NV_E4M3);
         return lo | hi << 16;
@@ -246,10 +257,8 @@ __device__ __forceinline__ uint32_t encode4(const float v[4], float inv, bool e4
     for (int i = 0; i < 4; ++i) r[i] = __float_as_uint(x[i]);
     if (bad)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (inv == 0x1p-122f) r[i] = __float_as_uint(fminf(fmaxf(x[i], 12582912.0f - 63.f), 12582912.0f + 63.f));
+        for (int i = 0; i < 4; ++i)
             if (abs_bits(v[i]) >= 0x7f800000u) r[i] = 0x80u;
-        }
     return __byte_perm(__byte_perm(r[0], r[1], 0x0040), __byte_perm(r[2], r[3], 0x0040), 0x5410);
 }
 
@@ -296,9 +305,10 @@ __device__ __forceinline__ uint32_t load_codes(const uint8_t* p, int n) {
     return w;
 }
 
-// quantise and store one block held by a warp; returns the scale's bits (the caller stores it)
+// quantise and store one block held by a warp, whose values are limited on the way; returns the scale's
+// bits (the caller stores it)
 template <bool VEC>
-__device__ __forceinline__ uint32_t store_block(uint8_t* p, int n, const float v[4], bool e4m3) {
+__device__ __forceinline__ uint32_t store_block(uint8_t* p, int n, float v[4], bool e4m3) {
     const Top t = warp_top(v, e4m3);
     const uint32_t s = scale_bits(t.bits, e4m3);
     store_codes<VEC>(p, n, encode4(v, inverse_pow2(s), e4m3, t.bad));

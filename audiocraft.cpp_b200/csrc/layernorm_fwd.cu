@@ -88,14 +88,15 @@ __global__ void __launch_bounds__(W * G * 32) ln_fwd_kernel(const FwdParams p) {
             p.rstd[row] = rstd;
         }
         if (KEEP) {
-            // a value that is not finite, or beyond 2^127, makes the sum of squares infinite or NaN unless it is
-            // close to the mean: one test a row
-            const bool bad = !(sq < __int_as_float(0x7f800000) && fabsf(mean) < 0x1p126f);
+            // one test a row: a value that is not finite or beyond the limit makes the sum of squares infinite or
+            // NaN, unless it is the mean (one column)
+            const bool bad = !(fmaf(mean, mean, sq) < __int_as_float(0x7f800000));
             uint32_t scale = 0;
 #pragma unroll
             for (int k = 0; k < NCH; ++k) {
                 float f[4];
                 unpairs(v[k], f);
+                if (bad) limit4(f, KEEP == 2);
                 const uint32_t s =
                     scale_bits(__reduce_max_sync(FULL_WARP, bad ? largest_finite(f) : largest(f)), KEEP == 2);
                 store_codes<VEC>(x8 + k * W * BLOCK, left - k * W * BLOCK, encode4(f, inverse_pow2(s), KEEP == 2, bad));

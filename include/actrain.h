@@ -341,9 +341,9 @@ int act_lora_linear(int device, const float* x, int64_t rows, int in, int out, i
  * An 8-bit tensor is codes and scales.  A block is 128 neighbouring columns (the last one of a
  * row may be shorter) of one row, or of 128 rows for a weight, and has one fp32 scale: the
  * smallest power of two s >= 2^-126 with |x| <= top * s for every finite x of the block (top 448
- * for E4M3, 127 for I8; an all-zero block has 2^-126).  A code is x / s rounded to nearest even (the
- * code below where that stands for 2^128, so that finite values stay finite in fp32), which is exact
- * arithmetic: codes and scales depend on x alone.  Relative to a free scale the
+ * for E4M3, 127 for I8; an all-zero block has 2^-126).  A code is x / s rounded to nearest even,
+ * which is exact arithmetic: codes and scales depend on x alone.  Finite values beyond 240 * 2^120 (E4M3) or
+ * 127 * 2^121 (I8), the largest that stay finite in fp32, count as those.  Relative to a free scale the
  * power of two costs E4M3 nothing but subnormal range, and I8 at most one bit.  A value that is
  * not finite is stored as NaN (E4M3 code 0x7f, I8 code -128) and leaves its block's scale alone.
  * Scales lie block-major, scale[(column / 128) * lds + row] (row / 128 for blocks of 128 rows):

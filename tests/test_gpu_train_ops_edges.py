@@ -59,17 +59,11 @@ def test_infinite_u_gives_what_the_formula_gives(rows, cols, nb, ut, kind):
 
 
 def nearest_kept(x, kind, block=1):
-    """Codes and scales of the definition, and what they stand for; a value that rounds to 2^128, which fp32
-    does not have, takes the code below."""
+    """Codes and scales of the definition, and what they stand for; finite values are limited first to the
+    largest that a code and a scale stand for in fp32 (the next code would be 2^128)."""
+    limit = 127 * 2.0 ** 121 if kind == A.CKPT_I8 else 240 * 2.0 ** 120
+    x = np.where(np.isfinite(x), np.clip(x, -limit, limit), x)
     q, s = E.encode(x, kind, block)
-    v = E.decode(q, s, kind, block)
-    past = np.abs(v) >= 2.0 ** 128
-    signed = q.view(np.int8).astype(np.int64)
-    if kind == A.CKPT_I8:
-        signed = np.where(past, signed - np.sign(signed), signed)
-        q = (signed & 255).astype(np.uint8)
-    else:
-        q = np.where(past, q - 1, q).astype(np.uint8)  # sign and size: one less is one step towards 0
     return q, s, E.decode(q, s, kind, block)
 
 
