@@ -1,5 +1,5 @@
 // ckpt8.cuh -- 8-bit tensors (codes and power-of-two block scales) and typed element access for
-// the kernels that write or read them: ckpt8.cu, layernorm.cu, rank_ckpt8.cu, gemm_f8.cu.
+// the kernels that write or read them: ckpt8.cu, layernorm_fwd.cu, layernorm_bwd.cu, rank_ckpt8.cu, gemm_f8.cu.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
@@ -321,7 +321,8 @@ __device__ __forceinline__ uint32_t store_block(uint8_t* p, int n, float v[4], b
 // 6.8e-8 for |z| <= 14.5, where Q leaves fp32's range; evaluated in fp32 5.6e-7 with a reciprocal
 // one step off) to exp(z^2 / 2) (1 - Phi(|z|)).  The form keeps relative accuracy in the tail,
 // where 1 - erf would cancel.  With the hardware's exponential (2^-22; it flushes below 2^-126) and
-// its argument's roundings (6.7e-8 z^2) the tail is within 2^-20 + 6.7e-8 z^2 of the true one.  Two values at a time: these passes are bound by issued instructions.
+// its argument's roundings (6.7e-8 z^2) the tail is within 2^-20 + 6.7e-8 z^2 of the true one.  Two
+// values at a time: half the instructions.
 __device__ __forceinline__ float ex2(float v) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));

@@ -7,18 +7,18 @@
 //   warp 0     TMA: raw codes into a ring of 64-row blocks
 //   warps 2, 3 U and the scales into the same ring (cp.async; loads to the converting warps' registers one
 //              block ahead came too late: 24000 x 6144, rank 16, f16 U 94 us, so 70)
-//   warps 8-15 codes * scale -> bf16 (exact: 4 or 7 significant bits times a power of two) in the
-//              128-byte-swizzled MN-major layout; the block's rows of U, cut into bf16 pieces that add
-//              up to it exactly (one for bf16, two for f16, three for fp32): both operands of the
-//              MMA have to be bf16, and the product keeps all of U
+//   warps 8-15 codes * scale -> bf16 (4 or 7 significant bits times a power of two: exact down to bf16's
+//              smallest step 2^-133) in the 128-byte-swizzled MN-major layout; the block's rows of U, cut
+//              into bf16 pieces that add up to it (one for bf16, two for f16, three for fp32; bits below
+//              2^-133 are cut off): both operands of the MMA have to be bf16, and the product keeps U
 //   warp 1     tcgen05 MMAs, the pieces side by side as their columns (one reading of the X tile feeds all)
 //   warps 4-7  the sums: the tensor cores cut each addition into the accumulator off below its last bit
 //              (measured: a relative 2^-24 downwards per 16 rows, 5e-6 over 4000 rows), so the
 //              accumulators are emptied into fp32 registers every 256 rows (two in turn where they fit)
 // The slices of a column tile form a cluster and add their sums in order through distributed
 // shared memory: no atomics, the same bits every time.
-// 24000 x 6144: rank 16 with f16 U 70 us (2.2 TB/s), rank 64 with bf16 U 90 us, with fp32 U 109 us
-// (shared memory and conversion take over from HBM).
+// 24000 x 6144 from E4M3 and I8: rank 16 with f16 U 70 us (2.2 TB/s) and 89 us, rank 64 with bf16 U 87 and
+// 90 us, with fp32 U 104 and 112 us (shared memory and conversion take over from HBM).
 #include <cuda.h>
 
 #include <atomic>
@@ -388,7 +388,7 @@ __global__ void __launch_bounds__(RTHREADS, 1) rank_kernel(const __grid_constant
             }
         }
         // Values at odd places are loaded by their own lane one block ahead: copies of 4 bytes keep warps 2
-        // and 3 longer (22317 x 25, fp32, rank 51: 37 us against 27).
+        // and 3 longer (22317 x 25 E4M3, fp32, rank 51: 37 us against 27).
         UnitOfU<U> un[NU];
         auto load = [&](int kb) {
 #pragma unroll

@@ -389,7 +389,8 @@ int64_t act_layernorm_bwd_workspace(int64_t rows, int64_t dim);
 
 /* GELU with the checkpoint of its input: g = z * Phi(z) (Phi the normal distribution function),
  * z8 receives z in 8 bits.  g may be NULL if g8 is given (fp32 result in 8 bits, as in
- * act_layernorm_fwd).  g_type equals z_type. */
+ * act_layernorm_fwd).  g has z's type.  Here and in the backward pass the normal tail is 0 where it would be
+ * below 2^-126 (z < -13.2). */
 int act_gelu_ckpt8_fwd(const void* z, int z_type, int64_t ldz, int64_t rows, int64_t cols, void* g, int64_t ldg,
                        const act_ckpt8* g8, const act_ckpt8* z8, void* stream);
 /* dz = dg * (Phi(z) + z * phi(z)) at the kept z; dz of dg's type may be NULL if dz8 is given. dz may
@@ -401,7 +402,7 @@ int act_gelu_ckpt8_bwd(const void* dg, int dg_type, int64_t lddg, const act_ckpt
  *   C[j][c] (+)= alpha * sum over rows t of U[t][j] * X[t][c],   C fp32 [nb][cols], 1 <= nb <= 64.
  * X in blocks of 1 row, its scales powers of two as act_ckpt8_store leaves them; its codes start on
  * 16-byte boundaries (q and ldq multiples of 16).  All of U's precision enters the product (fp32 U
- * included) and sums are fp32; infinities and NaN in U or X reach C as the formula has them.  accumulate
+ * included) and sums are fp32 (of U and X, what lies below 2^-133, bf16's smallest step, does not count); infinities and NaN in U or X reach C as the formula has them.  accumulate
  * 0 overwrites C.  status: a device int that the caller zeroes once and may read at any time; nonzero
  * means that a bounded wait inside the kernel ran out and C is not valid. */
 int act_rank_gemm_ckpt8(const void* u, int u_type, int64_t ldu, int nb, const act_ckpt8* x, int64_t rows,
