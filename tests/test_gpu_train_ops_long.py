@@ -258,7 +258,7 @@ def test_layernorm_backward_of_many_rows(rows, dim, t, kind):
 
 # ------------------------------------------------------------------------------ rank product
 # Blocks of 64 rows: sixteen slices of a narrow X (24000 rows: 23 or 24 blocks each, so five or six times
-# 256 rows and three turns of the ring), and 256 columns a block from 4737 columns on, seven slices of 18
+# 256 rows and three turns of the ring), and 256 columns a block from 4737 columns on, six slices of 21
 @pytest.mark.parametrize("rows,cols,nb", [(24001, 130, 16), (24001, 300, 64), (24001, 300, 5), (8003, 4900, 64),
                                           (8003, 4900, 17)])
 @pytest.mark.parametrize("kind", [A.CKPT_I8, A.CKPT_E4M3], ids=["i8", "e4m3"])
