@@ -5,12 +5,11 @@
 // bytes a block), load the reverse; the GELU's forward reads 2 and writes 2 + 1, its backward reads
 // 2 + 1 and writes 2 (16-bit types).  Store and load are bound by HBM.  GELU is short of both limits,
 // 77% of HBM's rate and 2.6 to 2.7 of 4 issues a cycle at a third of the warps: chains of dependent
-// arithmetic in few warps.  A warp
-// takes one block of 128 columns and RPW neighbouring rows of it at a time, with the next rows'
-// loads under way: a block's maximum is one warp reduction, and the rows' scales, which lie next to
-// each other (block-major), leave as one store.  GELU forward and backward of 12000 x 6144 bf16 with
-// E4M3 checkpoint: 149 us, 5.0 TB/s (167 us called in a loop); store and load of 6144 x 1536 fp32 in
-// 128 x 128 blocks: 14.8 us.
+// arithmetic in few warps.  A warp takes one block of 128 columns and RPW neighbouring rows of it at a
+// time, with the next rows' loads under way: a block's maximum is one warp reduction, and the rows'
+// scales, which lie next to each other (block-major), leave as one store.  GELU forward and backward of
+// 12000 x 6144 bf16 with E4M3 checkpoint: 149 us, 5.0 TB/s (167 us called in a loop); store and load of
+// 6144 x 1536 fp32 in 128 x 128 blocks: 14.8 us.
 #include <type_traits>
 
 #include "ckpt8.cuh"

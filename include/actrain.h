@@ -402,9 +402,10 @@ int act_gelu_ckpt8_bwd(const void* dg, int dg_type, int64_t lddg, const act_ckpt
  *   C[j][c] (+)= alpha * sum over rows t of U[t][j] * X[t][c],   C fp32 [nb][cols], 1 <= nb <= 64.
  * X in blocks of 1 row, its scales powers of two as act_ckpt8_store leaves them; its codes start on
  * 16-byte boundaries (q and ldq multiples of 16).  All of U's precision enters the product (fp32 U
- * included) and sums are fp32 (of U and X, what lies below 2^-133, bf16's smallest step, does not count); infinities and NaN in U or X reach C as the formula has them.  accumulate
- * 0 overwrites C.  status: a device int that the caller zeroes once and may read at any time; nonzero
- * means that a bounded wait inside the kernel ran out and C is not valid. */
+ * included) and sums are fp32 (of U and X, what lies below 2^-133, bf16's smallest step, does not count);
+ * infinities and NaN in U or X reach C as the formula has them.  accumulate 0 overwrites C.  status: a
+ * device int that the caller zeroes once and may read at any time; nonzero means that a bounded wait
+ * inside the kernel ran out and C is not valid. */
 int act_rank_gemm_ckpt8(const void* u, int u_type, int64_t ldu, int nb, const act_ckpt8* x, int64_t rows,
                         int64_t cols, float alpha, float* c, int64_t ldc, int accumulate, int32_t* status,
                         void* stream);
